@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define KCH_ABI_VERSION 23
+#define KCH_ABI_VERSION 24
 
 #define KCH_OK 0
 #define KCH_ERR_INVALID 1     /* bad pointer / shape / argument */
@@ -550,6 +550,94 @@ int kch_linear_rows(const void* x, long long ldx, const void* w, long long ldw, 
  */
 int kch_linear_up(const void* x, long long ldx, const void* w, long long ldw, void* y,
                   long long ldy, long long M, int N, int K, int dtype, void* stream);
+
+/* ---- The paged HCA cache ------------------------------------------------
+ * Sequences of unequal length over one pool of pages, for a serving loop: a
+ * step takes a chunk of new tokens of each of S sequences (single tokens are
+ * chunks of one), packed. (HCADecodingCache, ops_decoding_cache.py:1077-1395,
+ * holds equally long sequences and takes one token at a time.)
+ *
+ *   rows [P, page, c]      the pool, page a power of two up to 1024, c 64 or
+ *                          128, in `format`: 0 bf16, 1 e4m3 (OCP, no infinity), 2 int8
+ *   scales [P, page]       8-bit formats: E8M0 codes of the rows' scales, value
+ *                          = code 2^(scale code - 127); 255: the row is NaN
+ *   block_table [n_slots, nbp]  int32 page of a slot's compressed row b: entry
+ *                          b / page, line b % page
+ *   ring_table [n_slots, nrp]   int32 pages of its window rows: position p is
+ *                          ring row p % (nrp page), entry and line alike
+ *   slots [S], cu [S + 1], ctx [S]  int32: sequence i is slot slots[i], its
+ *                          tokens are packed rows cu[i] .. cu[i+1] - 1, the
+ *                          first of them at position ctx[i]
+ *
+ * All of them are device memory, read by the kernels alone: a captured step is
+ * replayed with new contents. Sequences that they do not describe rightly
+ * (rows outside 0 .. N - 1, a slot outside the tables, a negative position)
+ * are passed over. A table entry that names no page of the pool reads as a row of
+ * zeros and is not written. max_len is at least the longest chunk.
+ */
+
+/*
+ * A chunk's tokens into the cache: compressed rows of the blocks it ends
+ * (csa_compress_kv, ops_csa.py:198-234; per token,
+ * ops_decoding_cache.py:1200-1267) and the tokens' window rows, L2-normalised
+ * (normalize = 1) and quantised as they are written:
+ *   8-bit row x, amax = max |x|: scale 2^e, e the least integer with amax <=
+ *   448 2^e (e4m3) or 127 2^e (int8), 0 below 2^-100; code = rne(x / 2^e)
+ * C, Z [N, c] of dtype, rows ldc / ldz elements apart (16-byte aligned), B_pos
+ * [m2, c] fp32. state [n_slots, 3, c] fp32 holds, for the block that a slot's
+ * last token left open, the running max, sum and weighted sum of its softmax;
+ * it is read where ctx is inside a block and written where the chunk ends
+ * inside one. A slot may occur once. Window rows need max_len <= nrp page; to
+ * be read by the queries of their own chunk, win + max_len - 1 <= nrp page.
+ */
+int kch_hca_paged_append(const void* C, long long ldc, const void* Z, long long ldz, const float* B_pos,
+                         void* rows, void* scales, float* state, const int* block_table,
+                         const int* ring_table, const int* slots, const int* cu, const int* ctx, int S,
+                         int N, int c, int m2, int P, int page, int nbp, int nrp, int n_slots,
+                         int max_len, int normalize, int format, int dtype, void* stream);
+
+/*
+ * Attention of the chunk (whose tokens the cache holds already) over its
+ * sequence's cache, in one softmax with the sink (ops_hca.py:132-194): the
+ * query at position p sees the compressed rows b < (p + 1) / m2 and the window
+ * rows of positions max(0, p - win + 1) .. p; 0 where it sees none.
+ * q, out [N, nh, c] of dtype (contiguous, 16-byte aligned), sink [nh] fp32 or
+ * NULL; normalize_q: L2-normalise the queries. max_ctx is at least the largest
+ * ctx (it lays the work out; a larger one is answered rightly, if slower).
+ * Rows of out that belong to no sequence behind cu[S] are left as they were, or
+ * zeros with zero_tail. ws as kch_hca_paged_attn_ws_bytes says, 256-byte aligned.
+ */
+size_t kch_hca_paged_attn_ws_bytes(int S, int N, int nh, int c, int m2, int win, int max_len, int max_ctx);
+int kch_hca_paged_attn(const void* q, const float* sink, void* out, const void* rows, const void* scales,
+                       const int* block_table, const int* ring_table, const int* slots, const int* cu,
+                       const int* ctx, int S, int N, int nh, int c, int m2, int win, int P, int page,
+                       int nbp, int nrp, int n_slots, int max_len, int max_ctx, float scale,
+                       int normalize_q, int zero_tail, int format, int dtype, void* ws, size_t ws_bytes,
+                       void* stream);
+
+/*
+ * Cached rows back as numbers: output row cu[i] + j is row (first[i] + j) %
+ * (nbp page) of slot slots[i]'s pages in table [n_slots, nbp] (either table
+ * above; first NULL: 0). out [N, c] of odtype; rows behind cu[S] as above.
+ */
+int kch_paged_read(const void* rows, const void* scales, const int* table, const int* slots, const int* cu,
+                   const int* first, void* out, int S, int N, int c, int P, int page, int nbp, int n_slots,
+                   int zero_tail, int format, int odtype, void* stream);
+
+/*
+ * Few rows times a matrix of 4-bit weights with group scales, the layer
+ * projections of a decode step (kch_linear_rows) on a quarter of the bytes:
+ *   y[m, n] = sum_k x[m, k] scales[k / group, n] (code[n, k] - zeros[k / group, n])
+ *             (+ res[m, n])          (fp32 sums, rounded once)
+ * codes [N, K / 2] uint8, two a byte (low nibble: even k), 16-byte aligned;
+ * scales [K / group, N] of dtype (1 bf16, 2 fp16); zeros [K / group, N] uint8 or NULL
+ * (8). group 32, 64 or 128, K a multiple of it. x, res, y of dtype with row
+ * strides ldx (a multiple of 8, x 16-byte aligned), ldr, ldy. Any M >= 0; made for
+ * up to 16 rows (each further 16 read the weights again).
+ */
+int kch_linear_w4(const void* x, long long ldx, const void* codes, const void* scales, const void* zeros,
+                  const void* res, long long ldr, void* y, long long ldy, int M, int N, int K, int group,
+                  int dtype, void* stream);
 
 /* ---- Device-driven decode step ----------------------------------------
  * The entry points below make up one single-token decode step of

@@ -1545,6 +1545,147 @@ int kch_hca_decode_dyn(const void* q, long long ld_q, const void* kv_comp, long 
                          odtype, (char*)ws, (hipStream_t)stream, dyn);
 }
 
+// ---- The paged HCA cache and 4-bit weights ------------------------------------
+
+static int paged_pool(const char* fn, kch::PagedPool& pl, const void* rows, const void* scales,
+                      const int* block_table, const int* ring_table, const int* slots, const int* cu,
+                      const int* ctx, int S, int N, int c, int P, int page, int nbp, int nrp,
+                      int n_slots, int format) {
+  if (format < 0 || format > 2) return fail(KCH_ERR_INVALID, "%s: unknown page format %d", fn, format);
+  if (c != 64 && c != 128) return fail(KCH_ERR_UNSUPPORTED, "%s: c=%d not in {64, 128}", fn, c);
+  if (S < 0 || N < 0 || P < 0 || nbp < 0 || nrp < 0 || n_slots < 0)
+    return fail(KCH_ERR_INVALID, "%s: bad sizes S=%d N=%d P=%d nbp=%d nrp=%d n_slots=%d", fn, S, N, P,
+                nbp, nrp, n_slots);
+  if (S > 65534) return fail(KCH_ERR_UNSUPPORTED, "%s: S=%d sequences (at most 65534)", fn, S);
+  if (page < 1 || page > 1024 || (page & (page - 1)))
+    return fail(KCH_ERR_UNSUPPORTED, "%s: page=%d is not a power of two up to 1024", fn, page);
+  if ((long long)nbp * page > 0x7fffffffll || (long long)nrp * page > 0x7fffffffll)
+    return fail(KCH_ERR_UNSUPPORTED, "%s: a table of %d pages of %d rows", fn, nbp > nrp ? nbp : nrp, page);
+  if (S > 0 && N > 0) {
+    if (!slots || !cu || (n_slots > 0 && ((nbp > 0 && !block_table) || (nrp > 0 && !ring_table))))
+      return fail(KCH_ERR_INVALID, "%s: null table pointer", fn);
+    if (P > 0 && (!rows || (format != 0 && !scales))) return fail(KCH_ERR_INVALID, "%s: null pool pointer", fn);
+    if ((uintptr_t)rows & 15) return fail(KCH_ERR_INVALID, "%s: rows must be 16-byte aligned", fn);
+  }
+  pl.rows = const_cast<void*>(rows);
+  pl.scales = static_cast<uint8_t*>(const_cast<void*>(scales));
+  pl.block_table = block_table; pl.ring_table = ring_table;
+  pl.slots = slots; pl.cu = cu; pl.ctx = ctx;
+  pl.P = P; pl.nbp = nbp; pl.nrp = nrp; pl.n_slots = n_slots; pl.S = S; pl.N = N; pl.c = c;
+  pl.log2page = 0;
+  while ((1 << pl.log2page) < page) ++pl.log2page;
+  return KCH_OK;
+}
+
+int kch_hca_paged_append(const void* C, long long ldc, const void* Z, long long ldz, const float* B_pos,
+                         void* rows, void* scales, float* state, const int* block_table,
+                         const int* ring_table, const int* slots, const int* cu, const int* ctx, int S,
+                         int N, int c, int m2, int P, int page, int nbp, int nrp, int n_slots,
+                         int max_len, int normalize, int format, int dtype, void* stream) {
+  const char* fn = "kch_hca_paged_append";
+  kch::PagedAppendParams p;
+  int rc = paged_pool(fn, p.pool, rows, scales, block_table, ring_table, slots, cu, ctx, S, N, c, P, page,
+                      nbp, nrp, n_slots, format);
+  if (rc) return rc;
+  if (!dtype_ok(dtype)) return fail(KCH_ERR_INVALID, "%s: unknown dtype %d", fn, dtype);
+  if (m2 < 1 || max_len < 0) return fail(KCH_ERR_INVALID, "%s: bad m2=%d / max_len=%d", fn, m2, max_len);
+  if (nrp > 0 && max_len > (long long)nrp * page)
+    return fail(KCH_ERR_INVALID, "%s: max_len=%d exceeds the ring's %d rows", fn, max_len, nrp * page);
+  if (S == 0 || N == 0 || max_len == 0) return KCH_OK;
+  if (!C || !Z || !B_pos || !state || !ctx) return fail(KCH_ERR_INVALID, "%s: null pointer", fn);
+  const int es = dtype == KCH_DT_F32 ? 4 : 2;
+  if (ldc < c || ldz < c || (ldc * es) % 16 || (ldz * es) % 16 || ((uintptr_t)C | (uintptr_t)Z | (uintptr_t)B_pos) & 15)
+    return fail(KCH_ERR_INVALID, "%s: C, Z and B_pos rows must be 16-byte aligned", fn);
+  p.C = C; p.Z = Z; p.ldc = ldc; p.ldz = ldz; p.B_pos = B_pos; p.state = state;
+  p.m2 = m2; p.normalize = normalize; p.max_len = max_len < N ? max_len : N;
+  return hip_status(fn, kch::paged_append_dispatch(p, format, dtype, (hipStream_t)stream));
+}
+
+static bool paged_attn_sizes(int S, int N, int nh, int c, int m2, int win, int max_len, int max_ctx) {
+  return S >= 0 && N >= 0 && nh >= 1 && (c == 64 || c == 128) && m2 >= 1 && win >= 0 && max_len >= 0 &&
+         max_ctx >= 0 && (long long)N * nh < (1ll << 30);
+}
+
+size_t kch_hca_paged_attn_ws_bytes(int S, int N, int nh, int c, int m2, int win, int max_len, int max_ctx) {
+  if (!paged_attn_sizes(S, N, nh, c, m2, win, max_len, max_ctx) || S == 0 || N == 0 || max_len == 0) return 0;
+  return kch::paged_attn_plan(S, N, nh, c, m2, win, max_len < N ? max_len : N, max_ctx).bytes;
+}
+
+int kch_hca_paged_attn(const void* q, const float* sink, void* out, const void* rows, const void* scales,
+                       const int* block_table, const int* ring_table, const int* slots, const int* cu,
+                       const int* ctx, int S, int N, int nh, int c, int m2, int win, int P, int page,
+                       int nbp, int nrp, int n_slots, int max_len, int max_ctx, float scale,
+                       int normalize_q, int zero_tail, int format, int dtype, void* ws, size_t ws_bytes,
+                       void* stream) {
+  const char* fn = "kch_hca_paged_attn";
+  kch::PagedAttnParams p;
+  int rc = paged_pool(fn, p.pool, rows, scales, block_table, ring_table, slots, cu, ctx, S, N, c, P, page,
+                      nbp, nrp, n_slots, format);
+  if (rc) return rc;
+  if (!dtype_ok(dtype)) return fail(KCH_ERR_INVALID, "%s: unknown dtype %d", fn, dtype);
+  if (!paged_attn_sizes(S, N, nh, c, m2, win, max_len, max_ctx))
+    return fail(KCH_ERR_INVALID, "%s: bad sizes nh=%d m2=%d win=%d max_len=%d max_ctx=%d (N nh below 2^30)", fn,
+                nh, m2, win, max_len, max_ctx);
+  if (win > 0 && nrp > 0 && max_len > 0 && (long long)win + max_len - 1 > (long long)nrp * page)
+    return fail(KCH_ERR_INVALID, "%s: win=%d and max_len=%d exceed the ring's %d rows", fn, win, max_len,
+                nrp * page);
+  if (win > 0 && nrp == 0) return fail(KCH_ERR_INVALID, "%s: win=%d without a ring", fn, win);
+  if (N == 0 || ((S == 0 || max_len == 0) && !zero_tail)) return KCH_OK;
+  if (!q || !out || !slots || !cu || !ctx) return fail(KCH_ERR_INVALID, "%s: null pointer", fn);
+  if (((uintptr_t)q | (uintptr_t)out) & 15) return fail(KCH_ERR_INVALID, "%s: q and out must be 16-byte aligned", fn);
+  if (max_len > N) max_len = N;
+  if (max_len < 1) max_len = 1;
+  const kch::PagedAttnPlan pl = kch::paged_attn_plan(S, N, nh, c, m2, win, max_len, max_ctx);
+  if (pl.bytes) {
+    if (!ws || ws_bytes < pl.bytes) return fail(KCH_ERR_INVALID, "%s: workspace of %zu bytes required", fn, pl.bytes);
+    if ((uintptr_t)ws & 255) return fail(KCH_ERR_INVALID, "%s: workspace must be 256-byte aligned", fn);
+  }
+  p.q = q; p.sink = sink; p.out = out;
+  p.part_o = static_cast<float*>(ws);
+  p.part_ml = p.part_o ? p.part_o + (size_t)pl.nsplit * N * nh * c : nullptr;
+  p.nh = nh; p.m2 = m2; p.win = win; p.max_len = max_len; p.normalize_q = normalize_q;
+  p.zero_tail = zero_tail; p.nsplit = pl.nsplit; p.split_keys = pl.split_keys; p.scale = scale;
+  return hip_status(fn, kch::paged_attn_dispatch(p, pl, format, dtype, (hipStream_t)stream));
+}
+
+int kch_paged_read(const void* rows, const void* scales, const int* table, const int* slots, const int* cu,
+                   const int* first, void* out, int S, int N, int c, int P, int page, int nbp, int n_slots,
+                   int zero_tail, int format, int odtype, void* stream) {
+  const char* fn = "kch_paged_read";
+  kch::PagedReadParams p;
+  int rc = paged_pool(fn, p.pool, rows, scales, table, nullptr, slots, cu, first, S, N, c, P, page, nbp, 0,
+                      n_slots, format);
+  if (rc) return rc;
+  if (!dtype_ok(odtype)) return fail(KCH_ERR_INVALID, "%s: unknown dtype %d", fn, odtype);
+  if (N == 0 || (S == 0 && !zero_tail)) return KCH_OK;
+  if (!out || !cu) return fail(KCH_ERR_INVALID, "%s: null pointer", fn);
+  if ((uintptr_t)out & 15) return fail(KCH_ERR_INVALID, "%s: out must be 16-byte aligned", fn);
+  p.out = out;
+  p.zero_tail = zero_tail;
+  return hip_status(fn, kch::paged_read_dispatch(p, format, odtype, (hipStream_t)stream));
+}
+
+int kch_linear_w4(const void* x, long long ldx, const void* codes, const void* scales, const void* zeros,
+                  const void* res, long long ldr, void* y, long long ldy, int M, int N, int K, int group,
+                  int dtype, void* stream) {
+  const char* fn = "kch_linear_w4";
+  if (dtype != KCH_DT_BF16 && dtype != KCH_DT_F16)
+    return fail(KCH_ERR_UNSUPPORTED, "%s: dtype %d (bf16 or fp16 only)", fn, dtype);
+  if (M < 0 || N < 0 || K < 0) return fail(KCH_ERR_INVALID, "%s: bad sizes", fn);
+  if (group != 32 && group != 64 && group != 128)
+    return fail(KCH_ERR_UNSUPPORTED, "%s: group=%d not in {32, 64, 128}", fn, group);
+  if (K < group || K % group) return fail(KCH_ERR_UNSUPPORTED, "%s: K=%d not a multiple of group=%d", fn, K, group);
+  if (M == 0 || N == 0) return KCH_OK;
+  if (M > 16 * 65535) return fail(KCH_ERR_UNSUPPORTED, "%s: M=%d rows", fn, M);
+  if (!x || !codes || !scales || !y) return fail(KCH_ERR_INVALID, "%s: null pointer", fn);
+  if (ldx < K || ldy < N || (res && ldr < N)) return fail(KCH_ERR_INVALID, "%s: row strides below the row lengths", fn);
+  if (ldx % 8 || ((uintptr_t)x | (uintptr_t)codes) % 16)
+    return fail(KCH_ERR_UNSUPPORTED, "%s: rows of x and codes must be 16-byte aligned", fn);
+  kch::LinearW4Params p{x, static_cast<const uint8_t*>(codes), scales, static_cast<const uint8_t*>(zeros), res, y,
+                        ldx, ldr, ldy, M, N, K, group};
+  return hip_status(fn, kch::linear_w4_dispatch(p, dtype, (hipStream_t)stream));
+}
+
 }  // extern "C"
 
 // ---------------------------------------------------------------------------

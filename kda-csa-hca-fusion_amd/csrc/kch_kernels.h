@@ -424,6 +424,72 @@ hipError_t cache_step_dispatch(const CacheStepParams& p, int dtype, hipStream_t 
 hipError_t cache_step_rows_dispatch(const CacheStepParams& cp, const LinearRowsParams& lp, int dtype,
                                    hipStream_t s);
 
+// The paged HCA cache (paged_cache.hip, paged_attn.hip). A pool of P pages of
+// 2^log2page rows of c channels in one storage format, and per slot the pages of
+// its compressed rows (row b on page block_table[slot][b / page], line b % page)
+// and of its window rows (position p at ring row p % (nrp page)). A step: S
+// sequences, their slots, their packed tokens cu[i] .. cu[i+1] - 1 of N rows and
+// the tokens cached before them.
+enum PagedFormat : int { PF_BF16 = 0, PF_E4M3 = 1, PF_INT8 = 2 };
+struct PagedPool {
+  void* rows;             // [P, page, c]
+  uint8_t* scales;        // [P, page] E8M0 codes of the rows' scales (8-bit formats)
+  const int* block_table; // [n_slots, nbp]
+  const int* ring_table;  // [n_slots, nrp]
+  const int* slots;       // [S]
+  const int* cu;          // [S + 1]
+  const int* ctx;         // [S]
+  int P, log2page, nbp, nrp, n_slots, S, N, c;
+};
+struct PagedAppendParams {
+  PagedPool pool;
+  const void* C;          // [N, c] rows, ldc / ldz elements apart
+  const void* Z;
+  long long ldc, ldz;
+  const float* B_pos;     // [m2, c]
+  float* state;           // [n_slots, 3, c] running max, sum and weighted sum of the open block
+  int m2, normalize, max_len;
+};
+hipError_t paged_append_dispatch(const PagedAppendParams& p, int format, int dtype, hipStream_t s);
+struct PagedReadParams {
+  PagedPool pool;         // block_table: the table that is read; ctx: first row or null; N output rows
+  void* out;              // [N, c]
+  int zero_tail;          // rows behind the last sequence are written as zeros
+};
+hipError_t paged_read_dispatch(const PagedReadParams& p, int format, int odtype, hipStream_t s);
+struct PagedAttnParams {
+  PagedPool pool;
+  const void* q;          // [N, nh, c]
+  const float* sink;      // [nh] or null
+  void* out;              // [N, nh, c]
+  float* part_o;          // [nsplit, N nh, c] partial outputs (nsplit > 1)
+  float* part_ml;         // [nsplit, N nh, 2] their softmax reference and sum
+  int nh, m2, win, max_len, normalize_q, zero_tail, nsplit, split_keys;
+  float scale;
+};
+// How a call is laid out: query rows of a workgroup, key ranges and their length,
+// and the workspace that the ranges need.
+struct PagedAttnPlan {
+  int rows, nsplit, split_keys;
+  size_t bytes;
+};
+PagedAttnPlan paged_attn_plan(int S, int N, int nh, int c, int m2, int win, int max_len, int max_ctx);
+hipError_t paged_attn_dispatch(const PagedAttnParams& p, const PagedAttnPlan& plan, int format, int dtype,
+                               hipStream_t s);
+
+// Few rows times 4-bit weights (linear_w4.hip): y [M, N] = x [M, K] W^T (+ res), W[n, k] =
+// scales[k / group][n] (code - zeros[k / group][n]), codes [N, K / 2] two a byte.
+struct LinearW4Params {
+  const void* x;
+  const uint8_t* w;
+  const void* scales;     // [K / group, N] in x's type
+  const uint8_t* zeros;   // [K / group, N], or null: 8
+  const void* res;        // [M, N] or null
+  void* y;
+  long long ldx, ldr, ldy;
+  int M, N, K, group;     // group 32, 64 or 128; K a multiple of it
+};
+hipError_t linear_w4_dispatch(const LinearW4Params& p, int dtype, hipStream_t s);
 
 // Generic CSA / HCA forward (csa_hca_generic.hip): T = float or double
 // (f64), any head dims, indexer heads and indexer mask.

@@ -13,6 +13,8 @@ from .ops_csa import (csa_compress_kv, csa_compress_kv_overlapped, csa_core, rec
 from .ops_hca import hca_core, naive_hca
 from .ops_kda import kda_recurrent_grad, naive_chunk_kda, naive_recurrent_kda
 from .ops_kda_backend import hip_available, kda_forward, validate_kda_backend
+from .ops_w4 import W4Linear, linear_w4, quantize_w4
+from .paged import HCAPagedCache, hca_paged_append, hca_paged_attention, paged_read
 
 __all__ = [
     "CSAHybridLayer",
@@ -23,12 +25,19 @@ __all__ = [
     "KDAHybridLayer",
     "CSADecodingCache",
     "HCADecodingCache",
+    "HCAPagedCache",
     "SlidingWindowRingBuffer",
     "csa_compress_kv",
     "csa_compress_kv_overlapped",
     "csa_core",
     "kda_recurrent_grad",
     "hca_core",
+    "hca_paged_append",
+    "hca_paged_attention",
+    "linear_w4",
+    "paged_read",
+    "quantize_w4",
+    "W4Linear",
     "csa_lightning_indexer",
     "hip_available",
     "l2_normalize_rows",

@@ -88,6 +88,10 @@ _SIGNATURES = {
                           + [_I] * 5 + [_P, _SZ, _P],
     "kch_hca_decode_dyn": [_P, _L] * 3 + [_P, _I, _I, _I, _P, _P, _I, _I, _I, _F, _I, _I, _I,
                                           _P, _SZ, _P],
+    "kch_hca_paged_append": [_P, _L, _P, _L] + [_P] * 9 + [_I] * 13 + [_P],
+    "kch_hca_paged_attn": [_P] * 10 + [_I] * 13 + [_F] + [_I] * 4 + [_P, _SZ, _P],
+    "kch_paged_read": [_P] * 7 + [_I] * 10 + [_P],
+    "kch_linear_w4": [_P, _L] + [_P] * 4 + [_L, _P, _L] + [_I] * 5 + [_P],
 }
 
 # name -> (return type, argument types) of the entry points that return a value
@@ -102,6 +106,7 @@ _QUERIES = {
     "kch_csa_ste_bwd_ws_bytes": (_SZ, [_I] * 5),
     "kch_decode_ws_bytes": (_SZ, [_I] * 7),
     "kch_decode_dyn_ws_bytes": (_SZ, [_I] * 7),
+    "kch_hca_paged_attn_ws_bytes": (_SZ, [_I] * 8),
 }
 
 EXPORTED = ["kch_abi_version", "kch_last_error"] + sorted(_SIGNATURES) + sorted(_QUERIES)

@@ -1,0 +1,407 @@
+"""The paged HCA cache: sequences of unequal length, chunks of new tokens, 8-bit rows.
+
+``HCADecodingCache`` holds a batch of equally long sequences and takes one
+token a step. The operators here serve a changing set of sequences from one pool
+of pages:
+
+``hca_paged_append``     a chunk's tokens into the cache, quantised as they are written
+``hca_paged_attention``  the chunk's queries over it (``ops_hca.py:132-194``)
+``paged_read``           cached rows back as numbers
+``HCAPagedCache``        the pool, its page tables and the sequences in it
+
+A pool is ``rows [P, page, c]`` (bfloat16, float8_e4m3fn or int8) with, for the
+8-bit formats, ``scales [P, page]`` uint8: value = code * 2**(scale - 127), one
+power of two per row. ``block_table [n_slots, nbp]`` and ``ring_table [n_slots,
+nrp]`` (int32) give the pages of a slot's compressed rows and of its window rows
+(position p at ring row ``p % (nrp * page)``), ``state [n_slots, 3, c]`` fp32 the
+running softmax sums of its open block. A step names its sequences' ``slots
+[S]``, their packed tokens ``cu_seqlens [S + 1]`` and the tokens cached before
+them ``ctx_lens [S]``, int32 on the device. Only the sizes given as
+Python numbers enter the launches, so that a captured step replays with new
+contents of these tensors.
+
+Forward only, as the caches beside it.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .ops_csa import _HEAD_DIMS, _aligned, _f32_cached, _kernel_size, _pad_last
+
+_FORMATS = {torch.bfloat16: 0, torch.float8_e4m3fn: 1, torch.int8: 2}
+_I32 = torch.int32
+
+
+def _fail(fn, msg):
+    raise ValueError(f"{fn}: {msg}")
+
+
+def _ints(fn, name, t, dev, dims):
+    if t.dtype != _I32 or t.dim() != dims or not t.is_contiguous() or t.device != dev:
+        _fail(fn, f"{name} must be a contiguous int32 tensor of {dims} dimension(s) on {dev}, got "
+                  f"{t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _pool(fn, rows, scales):
+    """(format, P, page, c) of a pool after its checks."""
+    fmt = _FORMATS.get(rows.dtype)
+    if fmt is None:
+        raise TypeError(f"{fn}: rows must be bfloat16, float8_e4m3fn or int8, got {rows.dtype}")
+    if rows.dim() != 3 or not rows.is_contiguous():
+        _fail(fn, f"rows must be a contiguous [pages, page, c] tensor, got {tuple(rows.shape)}")
+    P, page, c = rows.shape
+    if fmt and (scales is None or scales.dtype != torch.uint8 or scales.shape != (P, page)
+                or not scales.is_contiguous() or scales.device != rows.device):
+        _fail(fn, f"8-bit rows need scales, contiguous uint8 [{P}, {page}] on {rows.device}")
+    return fmt, P, page, c
+
+
+def _step(fn, dev, slots, cu_seqlens, ctx_lens):
+    _ints(fn, "slots", slots, dev, 1)
+    _ints(fn, "cu_seqlens", cu_seqlens, dev, 1)
+    S = slots.shape[0]
+    if cu_seqlens.shape[0] != S + 1:
+        _fail(fn, f"cu_seqlens has {cu_seqlens.shape[0]} entries for {S} sequences")
+    if ctx_lens is not None:
+        _ints(fn, "ctx_lens", ctx_lens, dev, 1)
+        if ctx_lens.shape[0] != S:
+            _fail(fn, f"ctx_lens has {ctx_lens.shape[0]} entries for {S} sequences")
+    return S
+
+
+def _tables(fn, dev, block_table, ring_table):
+    _ints(fn, "block_table", block_table, dev, 2)
+    n_slots, nbp = block_table.shape
+    if ring_table is None:
+        return n_slots, nbp, 0
+    _ints(fn, "ring_table", ring_table, dev, 2)
+    if ring_table.shape[0] != n_slots:
+        _fail(fn, f"ring_table has {ring_table.shape[0]} slots, block_table {n_slots}")
+    return n_slots, nbp, ring_table.shape[1]
+
+
+def _rows2d(x):
+    """``x`` ``[N, c]`` with 16-byte aligned rows, and their stride."""
+    es = x.element_size()
+    if x.stride(1) != 1 or (x.stride(0) * es) % 16 or x.data_ptr() % 16 or x.stride(0) < x.shape[1]:
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x, x.stride(0)
+
+
+def _on(dev):
+    """Makes ``dev`` the current device of a launch where it is not."""
+    return torch.cuda.device(dev)
+
+
+def hca_paged_append(C, Z, B_pos, rows, scales, state, block_table, ring_table, slots, cu_seqlens,
+                     ctx_lens, *, m2, max_len, normalize=True):
+    """A chunk of tokens per sequence into the paged cache, in place.
+
+    ``C, Z`` ``[N, c]`` the packed tokens' projections (rows may be strided views),
+    ``B_pos [m2, c]``. Written: the compressed row of every block that the chunk
+    ends, each token's window row (with a ``ring_table``), both L2-normalised
+    (``normalize``) and quantised, and ``state`` where the chunk ends inside a
+    block. ``max_len`` is at least the longest chunk and at most the ring's rows; a slot
+    may occur once.
+    """
+    fn = "hca_paged_append"
+    _lib.require_gpu(fn, C, Z, rows)
+    fmt, P, page, c = _pool(fn, rows, scales)
+    dev = rows.device
+    if C.dim() != 2 or C.shape != Z.shape or C.shape[1] != c or C.dtype != Z.dtype or C.device != dev \
+            or Z.device != dev:
+        _fail(fn, f"C and Z must be [N, {c}] of one dtype on {dev}, got {tuple(C.shape)} {C.dtype} and "
+                  f"{tuple(Z.shape)} {Z.dtype}")
+    if m2 < 1:
+        _fail(fn, f"m2={m2} must be >= 1")
+    if B_pos.shape != (m2, c):
+        _fail(fn, f"B_pos.shape={tuple(B_pos.shape)} must equal (m2, c)=({m2}, {c})")
+    n_slots, nbp, nrp = _tables(fn, dev, block_table, ring_table)
+    if state.dtype != torch.float32 or state.shape != (n_slots, 3, c) or not state.is_contiguous() \
+            or state.device != dev:
+        _fail(fn, f"state must be contiguous float32 [{n_slots}, 3, {c}] on {dev}")
+    S = _step(fn, dev, slots, cu_seqlens, ctx_lens)
+    if max_len < 0 or (nrp and max_len > nrp * page):
+        _fail(fn, f"max_len={max_len} must be at most the ring's {nrp * page} rows")
+    code = _lib.dtype_code(fn, C.dtype)
+    C, ldc = _rows2d(C.detach())
+    Z, ldz = _rows2d(Z.detach())
+    B_pos = _aligned(_f32_cached(B_pos, dev))
+    ptr = _lib.ptr
+    with _on(dev):
+        _lib.call("kch_hca_paged_append", ptr(C), ldc, ptr(Z), ldz, ptr(B_pos), ptr(rows), ptr(scales),
+                  ptr(state), ptr(block_table), ptr(ring_table), ptr(slots), ptr(cu_seqlens),
+                  ptr(ctx_lens), S, C.shape[0], c, m2, P, page, nbp, nrp, n_slots, max_len,
+                  int(normalize), fmt, code, _lib.stream_of(rows))
+
+
+def hca_paged_attention(q, rows, scales, block_table, ring_table, slots, cu_seqlens, ctx_lens, *, m2,
+                        sliding_window, max_len, max_ctx=None, sink_logits=None, scale=1.0,
+                        normalize_q=True, out=None):
+    """Attention of each sequence's chunk over its cache, which holds the chunk already.
+
+    ``q`` ``[N, nh, c]`` the packed tokens' queries. The query at position p sees the
+    compressed rows ``b < (p + 1) // m2`` and the window rows of positions
+    ``max(0, p - sliding_window + 1) .. p`` in one softmax with the sink; 0 where it
+    sees none. ``max_len`` is at least the longest chunk, ``max_ctx`` at least the largest
+    of ``ctx_lens`` (it lays the work out). Returns ``[N, nh, c]`` in ``q.dtype``, or
+    writes ``out``; rows behind the last sequence are zeros, in ``out`` as they were.
+    The products are bf16 with fp32 sums whatever ``q``'s type.
+    """
+    fn = "hca_paged_attention"
+    _lib.require_gpu(fn, q, rows)
+    fmt, P, page, c = _pool(fn, rows, scales)
+    dev = rows.device
+    if q.dim() != 3 or q.shape[2] != c or q.shape[1] < 1 or q.device != dev:
+        _fail(fn, f"q must be [N, nh, {c}] on {dev}, got {tuple(q.shape)} on {q.device}")
+    N, nh, _ = q.shape
+    code = _lib.dtype_code(fn, q.dtype)
+    if m2 < 1:
+        _fail(fn, f"m2={m2} must be >= 1")
+    if sliding_window < 0:
+        _fail(fn, f"sliding_window={sliding_window} must be >= 0 (0 disables the branch)")
+    n_slots, nbp, nrp = _tables(fn, dev, block_table, ring_table)
+    S = _step(fn, dev, slots, cu_seqlens, ctx_lens)
+    if max_len < 0 or (sliding_window and sliding_window + max_len - 1 > nrp * page):
+        _fail(fn, f"sliding_window={sliding_window} and max_len={max_len} need a ring of "
+                  f"{sliding_window + max_len - 1} rows, it has {nrp * page}")
+    if max_ctx is None:
+        max_ctx = nbp * page * m2
+    if max_ctx < 0:
+        _fail(fn, f"max_ctx={max_ctx} must be >= 0")
+    max_ctx = min(max_ctx, 2 ** 31 - 1)
+    sink = None
+    if sink_logits is not None:
+        if sink_logits.shape != (nh,):
+            _fail(fn, f"sink_logits.shape={tuple(sink_logits.shape)} must equal (nh,)=({nh},)")
+        sink = _f32_cached(sink_logits, dev)
+    tail = out is None
+    if tail:
+        out = torch.empty(N, nh, c, device=dev, dtype=q.dtype)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous() \
+            or out.data_ptr() % 16:
+        _fail(fn, f"out must be a contiguous, 16-byte aligned {tuple(q.shape)} {q.dtype} tensor on {dev}")
+    q = _aligned(q.detach())
+    ptr = _lib.ptr
+    nbytes = _lib.load().kch_hca_paged_attn_ws_bytes(S, N, nh, c, m2, sliding_window, max_len, max_ctx)
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+    with _on(dev):
+        _lib.call("kch_hca_paged_attn", ptr(q), ptr(sink), ptr(out), ptr(rows), ptr(scales),
+                  ptr(block_table), ptr(ring_table), ptr(slots), ptr(cu_seqlens), ptr(ctx_lens), S, N, nh,
+                  c, m2, sliding_window, P, page, nbp, nrp, n_slots, max_len, max_ctx, float(scale),
+                  int(normalize_q), int(tail), fmt, code, ptr(ws), nbytes, _lib.stream_of(rows))
+    return out
+
+
+def paged_read(rows, scales, table, slots, cu_rows, *, total, first=None, dtype=torch.bfloat16, out=None):
+    """Rows of a paged cache as numbers, packed: row ``cu_rows[i] + j`` of the result is
+    row ``(first[i] + j) % capacity`` of slot ``slots[i]`` in ``table`` (a block or a ring
+    table), capacity its pages times their rows. ``total`` is the number of result rows; those
+    behind the last sequence are zeros (in ``out`` as they were)."""
+    fn = "paged_read"
+    _lib.require_gpu(fn, rows)
+    fmt, P, page, c = _pool(fn, rows, scales)
+    dev = rows.device
+    _ints(fn, "table", table, dev, 2)
+    S = _step(fn, dev, slots, cu_rows, first)
+    if total < 0:
+        _fail(fn, f"total={total} must be >= 0")
+    tail = out is None
+    if tail:
+        out = torch.empty(total, c, device=dev, dtype=dtype)
+    elif out.shape != (total, c) or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
+        _fail(fn, f"out must be a contiguous, 16-byte aligned [{total}, {c}] tensor on {dev}")
+    code = _lib.dtype_code(fn, out.dtype)
+    ptr = _lib.ptr
+    with _on(dev):
+        _lib.call("kch_paged_read", ptr(rows), ptr(scales), ptr(table), ptr(slots), ptr(cu_rows), ptr(first),
+                  ptr(out), S, total, c, P, page, table.shape[1], table.shape[0], int(tail), fmt, code,
+                  _lib.stream_of(rows))
+    return out
+
+
+class HCAPagedCache:
+    """HCA decode state of a changing set of sequences over one pool of pages.
+
+    ``add()`` opens a sequence and returns its slot, ``append_step`` takes a chunk of
+    new tokens of some sequences, ``forward_step`` their queries, ``release`` gives a
+    sequence's pages back. ``max_tokens`` bounds a sequence's length, ``max_chunk``
+    the tokens a step takes of one. Widths between the kernels' own are held
+    zero-padded. A single-threaded object on one stream, as the other caches.
+    """
+
+    def __init__(self, n_pages, c, m2, win, *, max_seqs, max_tokens, max_chunk=1, page=64,
+                 kv_dtype=torch.float8_e4m3fn, normalize_qk=True, device="cuda"):
+        fn = "HCAPagedCache"
+        for name, v, least in (("n_pages", n_pages, 1), ("c", c, 1), ("m2", m2, 1), ("win", win, 0),
+                               ("max_seqs", max_seqs, 1), ("max_tokens", max_tokens, 1),
+                               ("max_chunk", max_chunk, 1)):
+            if v < least:
+                _fail(fn, f"{name}={v} must be >= {least}")
+        if page < 1 or page > 1024 or page & (page - 1):
+            _fail(fn, f"page={page} must be a power of two up to 1024")
+        if kv_dtype not in _FORMATS:
+            raise TypeError(f"{fn}: kv_dtype must be bfloat16, float8_e4m3fn or int8, got {kv_dtype}")
+        if max_tokens >= 2 ** 31:
+            _fail(fn, f"max_tokens={max_tokens} must be below 2**31")
+        self.c, self.m2, self.win, self.page = c, m2, win, page
+        self.width = _kernel_size(fn, "c", c, _HEAD_DIMS)
+        self.max_tokens, self.max_chunk = max_tokens, max_chunk
+        self.normalize_qk = normalize_qk
+        self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None and torch.cuda.is_available():
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        nbp = -(-max(1, max_tokens // m2) // page)
+        nrp = -(-(win + max_chunk - 1) // page) if win else 0
+        kw = {"device": self.device}
+        self.rows = torch.zeros(n_pages, page, self.width, dtype=torch.uint8 if kv_dtype != torch.bfloat16
+                                else kv_dtype, **kw)
+        if kv_dtype != torch.bfloat16:
+            self.rows = self.rows.view(kv_dtype)
+        self.scales = None if kv_dtype == torch.bfloat16 else \
+            torch.full((n_pages, page), 127, dtype=torch.uint8, **kw)
+        self.state = torch.zeros(max_seqs, 3, self.width, dtype=torch.float32, **kw)
+        self.block_table = torch.full((max_seqs, nbp), -1, dtype=_I32, **kw)
+        self.ring_table = torch.full((max_seqs, nrp), -1, dtype=_I32, **kw) if win else None
+        self._free_pages = list(range(n_pages - 1, -1, -1))
+        self._free_slots = list(range(max_seqs - 1, -1, -1))
+        self._len = {}     # slot -> tokens cached
+        self._pages = {}   # slot -> (ring pages, block pages)
+        self._last = None  # the step that forward_step answers
+
+    @property
+    def n_free_pages(self) -> int:
+        return len(self._free_pages)
+
+    def n_tokens(self, slot) -> int:
+        return self._len[self._slot("n_tokens", slot)]
+
+    def n_blocks(self, slot) -> int:
+        return self.n_tokens(slot) // self.m2
+
+    def _slot(self, fn, slot):
+        if slot not in self._len:
+            _fail(f"HCAPagedCache.{fn}", f"slot {slot!r} holds no sequence")
+        return slot
+
+    def _upload(self, *lists):
+        """int32 lists on the device, in one copy."""
+        flat = [v for x in lists for v in x]
+        t = torch.tensor(flat, dtype=_I32, pin_memory=True).to(self.device, non_blocking=True)
+        return t.split([len(x) for x in lists])
+
+    def _take(self, fn, n):
+        if n > len(self._free_pages):
+            raise RuntimeError(f"HCAPagedCache.{fn}: {n} pages needed, {len(self._free_pages)} are free")
+        return [self._free_pages.pop() for _ in range(n)]
+
+    def add(self) -> int:
+        """Opens a sequence and returns its slot."""
+        if not self._free_slots:
+            raise RuntimeError("HCAPagedCache.add: every slot holds a sequence")
+        ring = self._take("add", 0 if self.ring_table is None else self.ring_table.shape[1])
+        slot = self._free_slots.pop()
+        if ring:
+            self.ring_table[slot] = self._upload(ring)[0]
+        self._len[slot], self._pages[slot] = 0, (ring, [])
+        return slot
+
+    def release(self, slot) -> None:
+        """Ends a sequence: its pages and its slot are free again."""
+        self._slot("release", slot)
+        ring, blocks = self._pages.pop(slot)
+        del self._len[slot]
+        self._free_pages += ring + blocks
+        self._free_slots.append(slot)
+        if self._last is not None and slot in self._last[0]:
+            self._last = None
+
+    def append_step(self, slots, C_new, Z_new, B_pos, lens=None):
+        """Appends ``lens[i]`` tokens (1 each by default) to sequence ``slots[i]``:
+        ``C_new, Z_new`` ``[sum(lens), c]``, packed in that order."""
+        fn = "append_step"
+        slots = list(slots)
+        lens = [1] * len(slots) if lens is None else list(lens)
+        if len(lens) != len(slots) or len(set(slots)) != len(slots):
+            _fail(f"HCAPagedCache.{fn}", "one length for each slot, and each slot once")
+        need = {}
+        for s, n in zip(slots, lens):
+            self._slot(fn, s)
+            if not 0 <= n <= self.max_chunk:
+                _fail(f"HCAPagedCache.{fn}", f"a chunk of {n} tokens (max_chunk={self.max_chunk})")
+            if self._len[s] + n > self.max_tokens:
+                _fail(f"HCAPagedCache.{fn}", f"slot {s} would hold {self._len[s] + n} tokens "
+                                             f"(max_tokens={self.max_tokens})")
+            k = -(-((self._len[s] + n) // self.m2) // self.page) - len(self._pages[s][1])
+            if k > 0:
+                need[s] = k
+        if C_new.dim() != 2 or C_new.shape != Z_new.shape or C_new.shape != (sum(lens), self.c):
+            _fail(f"HCAPagedCache.{fn}", f"C_new and Z_new must be [{sum(lens)}, {self.c}], got "
+                                         f"{tuple(C_new.shape)} and {tuple(Z_new.shape)}")
+        _lib.require_gpu(f"HCAPagedCache.{fn}", C_new, Z_new)
+        _lib.dtype_code(f"HCAPagedCache.{fn}", C_new.dtype)
+        if tuple(B_pos.shape) != (self.m2, self.c):
+            _fail(f"HCAPagedCache.{fn}", f"B_pos.shape={tuple(B_pos.shape)} must equal "
+                                         f"({self.m2}, {self.c})")
+        pages = self._take(fn, sum(need.values()))
+        at = []
+        for s, k in need.items():
+            have = self._pages[s][1]
+            at += [s * self.block_table.shape[1] + len(have) + i for i in range(k)]
+            have += pages[len(at) - k:len(at)]
+        ctx = [self._len[s] for s in slots]
+        cu = [0]
+        for n in lens:
+            cu.append(cu[-1] + n)
+        where, what, slots_d, cu_d, ctx_d = self._upload(at, pages, slots, cu, ctx)
+        if at:
+            self.block_table.view(-1)[where.long()] = what
+        with torch.no_grad():
+            hca_paged_append(_pad_last(C_new, self.width), _pad_last(Z_new, self.width),
+                             _pad_last(B_pos, self.width), self.rows, self.scales, self.state,
+                             self.block_table, self.ring_table, slots_d, cu_d, ctx_d, m2=self.m2,
+                             max_len=max(lens, default=0), normalize=self.normalize_qk)
+        for s, n in zip(slots, lens):
+            self._len[s] += n
+        self._last = (slots, slots_d, cu_d, ctx_d, cu[-1], max(lens, default=0), max(ctx, default=0))
+
+    def forward_step(self, q, *, scale=None, sink_logits=None, normalize_q=None):
+        """``[N, nh, c]`` in ``q.dtype``: the queries of the last ``append_step``'s tokens."""
+        fn = "HCAPagedCache.forward_step"
+        if self._last is None:
+            _fail(fn, "append_step first")
+        _, slots, cu, ctx, n, max_len, max_ctx = self._last
+        if q.dim() != 3 or q.shape[0] != n or q.shape[2] != self.c:
+            _fail(fn, f"q must be [{n}, nh, {self.c}], got {tuple(q.shape)}")
+        if scale is None:
+            scale = 1.0 if self.normalize_qk else self.c ** -0.5
+        with torch.no_grad():
+            out = hca_paged_attention(
+                _pad_last(q, self.width), self.rows, self.scales, self.block_table, self.ring_table, slots,
+                cu, ctx, m2=self.m2, sliding_window=self.win, max_len=max_len, max_ctx=max_ctx,
+                sink_logits=sink_logits, scale=scale,
+                normalize_q=self.normalize_qk if normalize_q is None else normalize_q)
+        return out if self.width == self.c else out[..., :self.c]
+
+    def read_blocks(self, slot, dtype=torch.bfloat16):
+        """The compressed rows ``[n_blocks, c]`` of a sequence."""
+        n = self.n_blocks(self._slot("read_blocks", slot))
+        s, cu = self._upload([slot], [0, n])
+        out = paged_read(self.rows, self.scales, self.block_table, s, cu, total=n, dtype=dtype)
+        return out[:, :self.c]
+
+    def read_window(self, slot, dtype=torch.bfloat16):
+        """The window rows ``[min(win, tokens), c]`` of a sequence, oldest first."""
+        t = self.n_tokens(slot)
+        n = min(self.win, t)
+        if not n:
+            return torch.empty(0, self.c, device=self.device, dtype=dtype)
+        cap = self.ring_table.shape[1] * self.page
+        s, cu, first = self._upload([slot], [0, n], [(t - n) % cap])
+        out = paged_read(self.rows, self.scales, self.ring_table, s, cu, total=n, first=first, dtype=dtype)
+        return out[:, :self.c]
+
+
+__all__ = ["HCAPagedCache", "hca_paged_append", "hca_paged_attention", "paged_read"]
