@@ -57,88 +57,181 @@ __device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
   w[0] = c[0]; w[1] = c[1]; w[2] = d[0]; w[3] = d[1];
 }
 
-// KW waves share a 16-row tile of W and its K range, 128 k at a time in turn.
-template <typename T, int KW, int G, bool ZP>
+// What a wave holds of 128 consecutive k: its tiles' codes, x, and per group the scales
+// (4 of 16 bits) and zero points (4 bytes) of the lane's rows of y^T.
+template <int NT, int G> struct W4Piece {
+  uint4 w[NT], x[4];
+  uint2 s[128 / G][NT];
+  uint32_t z[128 / G][NT];
+};
+
+// A workgroup takes NT 16-row tiles of W, its KW waves the K range 128 k at a time in
+// turn. The tiles of a wave share x (at M = 16 its rows are four times a tile's codes) and
+// the tile of ones. x is read by whole 128-byte lines and changes places through the wave's
+// LDS: in the order of its MFMA operand, 64 bytes of each of 16 rows an instruction, it
+// bound the kernel (16 rows, N 4096, K 8192: 13.7 against 10.1 us). VEC: N is a multiple of 4,
+// four scales are one load. The loop has no load behind a branch: a wait there would drain
+// every load in flight (the same kernel with such loads took 145 us where it took 43).
+// At 16 rows, N 16384, K 8192 20 us, 3.5 TB/s; 13.8 us is what its 71 MB take at the rate of a
+// large copy. Past the stream it is the 56 vector instructions a tile and 128 k, mostly the
+// codes' unpacking.
+template <typename T, int NT, int KW, int G, bool ZP, bool VEC, bool KT>
 __global__ __launch_bounds__(64 * KW) void linear_w4_kernel(LinearW4Params p) {
   using W = W4Type<T>;
   typedef typename W::v8 v8;
-  constexpr int U = 2;      // 128-k pieces of a wave whose loads are in flight together
-  constexpr int SPG = G / 32;  // MFMA steps of a group
-  __shared__ float part[KW][16][17];
+  typedef W4Piece<NT, G> Piece;
+  constexpr int NG = 128 / G;
+  constexpr int XB = 4096, PB = 16 * (16 * NT + 1) * 4;  // bytes of a wave's x and of its partial tiles
+  __shared__ __attribute__((aligned(16))) char lds[KW * (XB > PB ? XB : PB)];
+  float (*const part)[16][16 * NT + 1] = reinterpret_cast<float (*)[16][16 * NT + 1]>(lds);
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int lane = lane_id(), r = lane & 15, q = lane >> 4;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
+  const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16;
   const int K = p.K, N = p.N;
-  // rows past N read row N - 1 again (never stored)
-  const uint4* wrow = reinterpret_cast<const uint4*>(p.w + (size_t)min(n0 + r, N - 1) * (K / 2)) + q;
-  const bool mok = m0 + r < p.M;
-  const T* xrow = static_cast<const T*>(p.x) + (size_t)(mok ? m0 + r : 0) * p.ldx + 8 * q;
-  const T* const sc = static_cast<const T*>(p.scales);
-  const int np = (K + 127) / 128;
-  const int ns = n0 + 4 * q;  // the lane's four rows of y^T
-  uint4 ones_w = make_uint4(W::one2, W::one2, W::one2, W::one2);
-  const v8 ones = __builtin_bit_cast(v8, ones_w);
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  const uint4 z4 = make_uint4(0, 0, 0, 0);
-  for (int p0 = wv; p0 < np; p0 += KW * U) {
-    uint4 wq[U], xq[U][4];
-    float s[U][4 / SPG][4], z[U][4 / SPG][4];
+  // rows past M and N read the last one again: their results are never stored
+  const T* const xa = static_cast<const T*>(p.x) + (size_t)min(m0 + lane / 8, p.M - 1) * p.ldx + 8 * (lane & 7);
+  const T* const xb = static_cast<const T*>(p.x) + (size_t)min(m0 + 8 + lane / 8, p.M - 1) * p.ldx + 8 * (lane & 7);
+  uint4* const xl = reinterpret_cast<uint4*>(lds) + 256 * wv;
+  const uint4* wrow[NT];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int pc = p0 + u * KW, k0 = 128 * pc;
-      wq[u] = pc < np && k0 + 32 * q < K ? wrow[4 * pc] : z4;
+  for (int t = 0; t < NT; ++t)
+    wrow[t] = reinterpret_cast<const uint4*>(p.w + (size_t)min(n0 + 16 * t + r, N - 1) * (K / 2)) + q;
+  const uint16_t* const sc = static_cast<const uint16_t*>(p.scales);
+
+  // TAIL: the last piece where K is no multiple of 128; what lies past K is read from
+  // inside the row and meets zeros of x
+  auto load = [&](Piece& c, int pc, auto tail) {
+    constexpr bool TAIL = decltype(tail)::value;
+    const int k0 = 128 * pc;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        xq[u][j] = mok && pc < np && k0 + 32 * j < K ? *reinterpret_cast<const uint4*>(xrow + k0 + 32 * j) : z4;
+    for (int t = 0; t < NT; ++t) c.w[t] = wrow[t][TAIL && k0 + 32 * q >= K ? -q : 4 * pc];
+    const int ka = k0 + 8 * (lane & 7), kb = ka + 64;  // this lane's k of its two lines
+    const bool pa = TAIL && ka >= K, pb = TAIL && kb >= K;
+    c.x[0] = *reinterpret_cast<const uint4*>(xa + (pa ? 0 : k0));
+    c.x[1] = *reinterpret_cast<const uint4*>(xa + (pb ? 0 : k0 + 64));
+    c.x[2] = *reinterpret_cast<const uint4*>(xb + (pa ? 0 : k0));
+    c.x[3] = *reinterpret_cast<const uint4*>(xb + (pb ? 0 : k0 + 64));
+    if (pa) c.x[0] = c.x[2] = make_uint4(0, 0, 0, 0);
+    if (pb) c.x[1] = c.x[3] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int g = 0; g < 4 / SPG; ++g) {
-        const int k = k0 + G * g;
+    for (int g = 0; g < NG; ++g) {
+      const size_t row = (size_t)(TAIL ? min(k0 / G + g, K / G - 1) : k0 / G + g) * N;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int n = n0 + 16 * t + 4 * q;
+        if constexpr (VEC) {
+          const size_t at = row + min(n, N - 4);
+          c.s[g][t] = *reinterpret_cast<const uint2*>(sc + at);
+          if constexpr (ZP) c.z[g][t] = *reinterpret_cast<const uint32_t*>(p.zeros + at);
+        } else {
+          uint32_t v[4], z = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const size_t at = row + min(n + e, N - 1);
+            v[e] = sc[at];
+            if constexpr (ZP) z |= (uint32_t)p.zeros[at] << (8 * e);
+          }
+          c.s[g][t] = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
+          if constexpr (ZP) c.z[g][t] = z;
+        }
+      }
+    }
+  };
+
+  const v8 ones = __builtin_bit_cast(v8, make_uint4(W::one2, W::one2, W::one2, W::one2));
+  f32x4 acc[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  auto use = [&](Piece& c) {
+    uint32_t w4[NT][4];
+    v8 bx[4];
+    wave_lds_sync();
+    const int ra = lane / 8, ch = lane & 7;
+    xl[16 * ra + (ch ^ ra)] = c.x[0];
+    xl[16 * ra + ((8 + ch) ^ ra)] = c.x[1];
+    xl[16 * (8 + ra) + (ch ^ (8 + ra))] = c.x[2];
+    xl[16 * (8 + ra) + ((8 + ch) ^ (8 + ra))] = c.x[3];
+    wave_lds_sync();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c.x[j] = xl[16 * r + ((4 * j + q) ^ r)];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      w4[t][0] = c.w[t].x; w4[t][1] = c.w[t].y; w4[t][2] = c.w[t].z; w4[t][3] = c.w[t].w;
+      transpose4(w4[t]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // codes (e, e + 4) of a word come out in the halves of register e: x alike
+      const uint4 x = c.x[j];
+      uint4 b;
+      b.x = __builtin_amdgcn_perm(x.z, x.x, 0x05040100u);
+      b.y = __builtin_amdgcn_perm(x.z, x.x, 0x07060302u);
+      b.z = __builtin_amdgcn_perm(x.w, x.y, 0x05040100u);
+      b.w = __builtin_amdgcn_perm(x.w, x.y, 0x07060302u);
+      bx[j] = __builtin_bit_cast(v8, b);
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      // sum x, and what the offset (and a zero point of 8) adds to every code: the
+      // products start from its negative
+      f32x4 sum = {0.f, 0.f, 0.f, 0.f}, base;
+#pragma unroll
+      for (int j = g * G / 32; j < (g + 1) * G / 32; ++j) sum = W::mfma(ones, bx[j], sum);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) base[e] = -(W::offset + (ZP ? 0.f : 8.f)) * sum[e];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        f32x4 raw = base;
+#pragma unroll
+        for (int j = g * G / 32; j < (g + 1) * G / 32; ++j) {
+          const uint32_t w = w4[t][j];
+          uint4 a;
+          a.x = (w & 0x000f000fu) | W::magic;
+          a.y = ((w >> 4) & 0x000f000fu) | W::magic;
+          a.z = ((w >> 8) & 0x000f000fu) | W::magic;
+          a.w = ((w >> 12) & 0x000f000fu) | W::magic;
+          raw = W::mfma(__builtin_bit_cast(v8, a), bx[j], raw);
+        }
+        const uint32_t sw[2] = {c.s[g][t].x, c.s[g][t].y};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool ok = pc < np && k < K;
-          const size_t at = (size_t)(ok ? k / G : 0) * N + min(ns + e, N - 1);
-          s[u][g][e] = ok ? to_f32(sc[at]) : 0.f;
-          z[u][g][e] = W::offset + (ZP ? (float)p.zeros[at] : 8.f);
+          const float s = to_f32(__builtin_bit_cast(T, (uint16_t)(sw[e >> 1] >> (16 * (e & 1)))));
+          const float d = ZP ? fmaf(-(float)((c.z[g][t] >> (8 * e)) & 255u), sum[e], raw[e]) : raw[e];
+          acc[t][e] = fmaf(s, d, acc[t][e]);
         }
       }
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      uint32_t w4[4] = {wq[u].x, wq[u].y, wq[u].z, wq[u].w};
-      transpose4(w4);
-      f32x4 raw = {0.f, 0.f, 0.f, 0.f}, sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        // codes (e, e + 4) of the word in the halves of register e, and x alike
-        uint4 a;
-        a.x = (w4[j] & 0x000f000fu) | W::magic;
-        a.y = ((w4[j] >> 4) & 0x000f000fu) | W::magic;
-        a.z = ((w4[j] >> 8) & 0x000f000fu) | W::magic;
-        a.w = ((w4[j] >> 12) & 0x000f000fu) | W::magic;
-        const uint4 x = xq[u][j];
-        uint4 b;
-        b.x = __builtin_amdgcn_perm(x.z, x.x, 0x05040100u);
-        b.y = __builtin_amdgcn_perm(x.z, x.x, 0x07060302u);
-        b.z = __builtin_amdgcn_perm(x.w, x.y, 0x05040100u);
-        b.w = __builtin_amdgcn_perm(x.w, x.y, 0x07060302u);
-        const v8 bv = __builtin_bit_cast(v8, b);
-        raw = W::mfma(__builtin_bit_cast(v8, a), bv, raw);
-        sum = W::mfma(ones, bv, sum);
-        if (j % SPG == SPG - 1) {
-          const int g = j / SPG;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] = fmaf(s[u][g][e], fmaf(-z[u][g][e], sum[e], raw[e]), acc[e]);
-          raw = sum = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-      }
+  };
+
+  // two pieces in turn: the next one's loads are in flight while one is used (past the
+  // end the last one again, from the cache); KT: K has a tail past its last 128, which
+  // comes first, beside the first piece (its code alone, unused, cost the large case 8%)
+  const std::integral_constant<bool, false> whole{};
+  const int nf = K / 128;
+  Piece c0, c1;
+  if (wv < nf) load(c0, wv, whole);
+  if (KT && wv == nf % KW) {
+    load(c1, nf, std::integral_constant<bool, true>{});
+    use(c1);
+  }
+  if (wv < nf) {
+    for (int pc = wv; pc < nf; pc += 2 * KW) {
+      load(c1, min(pc + KW, nf - 1), whole);
+      use(c0);
+      load(c0, min(pc + 2 * KW, nf - 1), whole);
+      if (pc + KW < nf) use(c1);
     }
   }
-  // acc[e]: y^T[n0 + 4 q + e][m0 + r]
+  __syncthreads();  // the partial tiles go where x was
+  // acc[t][e]: y^T[n0 + 16 t + 4 q + e][m0 + r]
 #pragma unroll
-  for (int e = 0; e < 4; ++e) part[wv][r][4 * q + e] = acc[e];
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[wv][r][16 * t + 4 * q + e] = acc[t][e];
   __syncthreads();
-  for (int t = threadIdx.x; t < 256; t += 64 * KW) {
-    const int m = t >> 4, n = t & 15;
+  for (int i = threadIdx.x; i < 256 * NT; i += 64 * KW) {
+    const int m = i / (16 * NT), n = i % (16 * NT);
     if (m0 + m >= p.M || n0 + n >= N) continue;
     float v = 0.f;
 #pragma unroll
@@ -148,25 +241,47 @@ __global__ __launch_bounds__(64 * KW) void linear_w4_kernel(LinearW4Params p) {
   }
 }
 
-template <typename T, int G>
+template <typename T, int NT, int G, bool VEC>
 void w4_launch(const LinearW4Params& p, hipStream_t s) {
-  const dim3 grid((unsigned)((p.N + 15) / 16), (unsigned)((p.M + 15) / 16));
-  if (p.zeros) hipLaunchKernelGGL((linear_w4_kernel<T, 4, G, true>), grid, dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((linear_w4_kernel<T, 4, G, false>), grid, dim3(256), 0, s, p);
+  const dim3 grid((unsigned)((p.N + 16 * NT - 1) / (16 * NT)), (unsigned)((p.M + 15) / 16)), block(512);
+#define KCH_W4(ZP, KT) hipLaunchKernelGGL((linear_w4_kernel<T, NT, 8, G, ZP, VEC, KT>), grid, block, 0, s, p)
+  if constexpr (G < 128) {
+    if (p.K % 128) {
+      if (p.zeros) KCH_W4(true, true);
+      else KCH_W4(false, true);
+      return;
+    }
+  }
+  if (p.zeros) KCH_W4(true, false);
+  else KCH_W4(false, false);
+#undef KCH_W4
 }
 
-template <typename T>
+template <typename T, int NT, bool VEC>
 void w4_launch_g(const LinearW4Params& p, hipStream_t s) {
-  if (p.group == 32) w4_launch<T, 32>(p, s);
-  else if (p.group == 64) w4_launch<T, 64>(p, s);
-  else w4_launch<T, 128>(p, s);
+  if (p.group == 32) w4_launch<T, NT, 32, VEC>(p, s);
+  else if (p.group == 64) w4_launch<T, NT, 64, VEC>(p, s);
+  else w4_launch<T, NT, 128, VEC>(p, s);
+}
+
+// Tiles of a workgroup of 8 waves (one a CU): as many as leave a workgroup for each of 256
+// CUs. Measured (us, bf16, groups of 128, weights from HBM) with 1 / 2 / 4 tiles: one row, N 2048,
+// K 2048 4.1 / 4.8 / 6.6; 16 rows, N 4096, K 8192 10.1 / 12.0 / 18.2, N 8192, K 2048 7.4 /
+// 6.2 / 8.9, N 16384, K 8192 29.1 / 22.1 / 20.3.
+template <typename T>
+void w4_launch_n(const LinearW4Params& p, hipStream_t s) {
+  const long long tiles = (long long)((p.N + 15) / 16) * ((p.M + 15) / 16);
+  if (p.N % 4 || ((uintptr_t)p.scales & 7) || ((uintptr_t)p.zeros & 3)) w4_launch_g<T, 1, false>(p, s);
+  else if (tiles >= 1024) w4_launch_g<T, 4, true>(p, s);
+  else if (tiles >= 512) w4_launch_g<T, 2, true>(p, s);
+  else w4_launch_g<T, 1, true>(p, s);
 }
 
 }  // namespace
 
 hipError_t linear_w4_dispatch(const LinearW4Params& p, int dtype, hipStream_t s) {
-  if (dtype == DT_BF16) w4_launch_g<bf16_t>(p, s);
-  else w4_launch_g<_Float16>(p, s);
+  if (dtype == DT_BF16) w4_launch_n<bf16_t>(p, s);
+  else w4_launch_n<_Float16>(p, s);
   return hipGetLastError();
 }
 

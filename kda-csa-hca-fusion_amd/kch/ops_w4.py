@@ -25,49 +25,54 @@ def linear_w4(x, packed, scales, zeros=None, *, residual=None):
     rounded once. The group is ``K / scales.shape[0]``. Made for the few rows of a decode
     step; any number is taken, each 16 reading the weights again."""
     fn = "linear_w4"
-    _lib.require_gpu(fn, x, packed)
-    dt, dev = x.dtype, x.device
-    if dt not in (torch.bfloat16, torch.float16):
+    if not (x.is_cuda and packed.is_cuda):
+        _lib.require_gpu(fn, x, packed)
+    dt, dev = x.dtype, x.get_device()
+    if dt is not torch.bfloat16 and dt is not torch.float16:
         raise TypeError(f"{fn}: x must be bfloat16 or float16, got {dt}")
-    if packed.dtype != torch.uint8 or packed.dim() != 2 or not packed.is_contiguous() or packed.device != dev:
-        raise ValueError(f"{fn}: packed must be a contiguous uint8 [N, K / 2] tensor on {dev}, got "
+    if packed.dtype is not torch.uint8 or packed.dim() != 2 or not packed.is_contiguous() \
+            or packed.get_device() != dev:
+        raise ValueError(f"{fn}: packed must be a contiguous uint8 [N, K / 2] tensor on {x.device}, got "
                          f"{packed.dtype} {tuple(packed.shape)}")
-    N, K = packed.shape[0], 2 * packed.shape[1]
+    N, K = packed.shape
+    K *= 2
     if x.dim() < 1 or x.shape[-1] != K:
         raise ValueError(f"{fn}: x {tuple(x.shape)} does not have the weights' K={K} columns")
-    if scales.dim() != 2 or scales.shape[1] != N or scales.dtype != dt or not scales.is_contiguous() \
-            or scales.device != dev:
-        raise ValueError(f"{fn}: scales must be a contiguous {dt} [K / group, {N}] tensor on {dev}, got "
+    if scales.dim() != 2 or scales.shape[1] != N or scales.dtype is not dt or not scales.is_contiguous() \
+            or scales.get_device() != dev:
+        raise ValueError(f"{fn}: scales must be a contiguous {dt} [K / group, {N}] tensor on {x.device}, got "
                          f"{scales.dtype} {tuple(scales.shape)}")
     ng = scales.shape[0]
     group = K // ng if ng and K % ng == 0 else 0
     if group not in _GROUPS:
         raise ValueError(f"{fn}: {ng} rows of scales for K={K}: a group has {_GROUPS} columns")
-    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape
-                              or not zeros.is_contiguous() or zeros.device != dev):
-        raise ValueError(f"{fn}: zeros must be a contiguous uint8 {tuple(scales.shape)} tensor on {dev}")
-    shape = (*x.shape[:-1], N)
-    x2 = x.detach().reshape(-1, K)
+    if zeros is not None and (zeros.dtype is not torch.uint8 or zeros.shape != scales.shape
+                              or not zeros.is_contiguous() or zeros.get_device() != dev):
+        raise ValueError(f"{fn}: zeros must be a contiguous uint8 {tuple(scales.shape)} tensor on {x.device}")
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
     M = x2.shape[0]
-    if x2.stride(1) != 1 or (M > 1 and (x2.stride(0) % 8 or x2.stride(0) < K)) or x2.data_ptr() % 16:
-        x2 = x2.clone(memory_format=torch.contiguous_format)
+    ldx, one = x2.stride()
+    if M == 1:
+        ldx = K
+    if one != 1 or ldx % 8 or ldx < K or x2.data_ptr() % 16:
+        x2 = x2.detach().clone(memory_format=torch.contiguous_format)
+        ldx = K
     if packed.data_ptr() % 16:
         packed = packed.clone()
+    y = torch.empty(*x.shape[:-1], N, device=x.device, dtype=dt)
     r2, ldr = None, 0
     if residual is not None:
-        if residual.shape != shape or residual.dtype != dt or residual.device != dev:
-            raise ValueError(f"{fn}: residual must be {shape} {dt} on {dev}, got {tuple(residual.shape)} "
-                             f"{residual.dtype}")
-        r2 = residual.detach().reshape(M, N)
-        if r2.stride(1) != 1 or r2.stride(0) < N:
-            r2 = r2.clone(memory_format=torch.contiguous_format)
-        ldr = max(r2.stride(0), N)
-    y = torch.empty(shape, device=dev, dtype=dt)
-    ptr = _lib.ptr
-    with torch.cuda.device(dev):
-        _lib.call("kch_linear_w4", ptr(x2), x2.stride(0) if M > 1 else K, ptr(packed), ptr(scales),
-                  ptr(zeros), ptr(r2), ldr, ptr(y), N, M, N, K, group, _lib.dtype_code(fn, dt),
-                  _lib.stream_of(x))
+        if residual.shape != y.shape or residual.dtype is not dt or residual.get_device() != dev:
+            raise ValueError(f"{fn}: residual must be {tuple(y.shape)} {dt} on {x.device}, got "
+                             f"{tuple(residual.shape)} {residual.dtype}")
+        r2 = residual if residual.dim() == 2 else residual.reshape(M, N)
+        ldr, one = r2.stride()
+        if one != 1 or ldr < N:
+            r2 = r2.detach().clone(memory_format=torch.contiguous_format)
+            ldr = N
+    _lib.call_on(dev, "kch_linear_w4", x2.data_ptr(), ldx, packed.data_ptr(), scales.data_ptr(),
+                 None if zeros is None else zeros.data_ptr(), None if r2 is None else r2.data_ptr(), ldr,
+                 y.data_ptr(), N, M, N, K, group, 1 if dt is torch.bfloat16 else 2)
     return y
 
 

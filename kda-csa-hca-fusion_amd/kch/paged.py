@@ -38,61 +38,78 @@ def _fail(fn, msg):
     raise ValueError(f"{fn}: {msg}")
 
 
-def _ints(fn, name, t, dev, dims):
-    if t.dtype != _I32 or t.dim() != dims or not t.is_contiguous() or t.device != dev:
-        _fail(fn, f"{name} must be a contiguous int32 tensor of {dims} dimension(s) on {dev}, got "
+# The checks of a step's tensors are single expressions over attributes of about 50 ns
+# each, with the message made only where one fails: a decode step pays them per layer.
+
+def _is_ints(t, dim, dev):
+    return t.dtype is _I32 and t.dim() == dim and t.is_contiguous() and t.get_device() == dev
+
+
+def _need_ints(fn, name, t, dim, dev):
+    if not _is_ints(t, dim, dev):
+        _fail(fn, f"{name} must be a contiguous int32 tensor of {dim} dimension(s) on cuda:{dev}, got "
                   f"{t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def _pool(fn, rows, scales):
-    """(format, P, page, c) of a pool after its checks."""
+    """(format, P, page, c, device index) of a pool after its checks."""
     fmt = _FORMATS.get(rows.dtype)
     if fmt is None:
         raise TypeError(f"{fn}: rows must be bfloat16, float8_e4m3fn or int8, got {rows.dtype}")
     if rows.dim() != 3 or not rows.is_contiguous():
         _fail(fn, f"rows must be a contiguous [pages, page, c] tensor, got {tuple(rows.shape)}")
     P, page, c = rows.shape
-    if fmt and (scales is None or scales.dtype != torch.uint8 or scales.shape != (P, page)
-                or not scales.is_contiguous() or scales.device != rows.device):
+    dev = rows.get_device()
+    if fmt and (scales is None or scales.dtype is not torch.uint8 or scales.shape != (P, page)
+                or not scales.is_contiguous() or scales.get_device() != dev):
         _fail(fn, f"8-bit rows need scales, contiguous uint8 [{P}, {page}] on {rows.device}")
-    return fmt, P, page, c
+    return fmt, P, page, c, dev
 
 
 def _step(fn, dev, slots, cu_seqlens, ctx_lens):
-    _ints(fn, "slots", slots, dev, 1)
-    _ints(fn, "cu_seqlens", cu_seqlens, dev, 1)
     S = slots.shape[0]
-    if cu_seqlens.shape[0] != S + 1:
-        _fail(fn, f"cu_seqlens has {cu_seqlens.shape[0]} entries for {S} sequences")
-    if ctx_lens is not None:
-        _ints(fn, "ctx_lens", ctx_lens, dev, 1)
-        if ctx_lens.shape[0] != S:
-            _fail(fn, f"ctx_lens has {ctx_lens.shape[0]} entries for {S} sequences")
+    if not (_is_ints(slots, 1, dev) and _is_ints(cu_seqlens, 1, dev) and cu_seqlens.shape[0] == S + 1
+            and (ctx_lens is None or (_is_ints(ctx_lens, 1, dev) and ctx_lens.shape[0] == S))):
+        for name, t in (("slots", slots), ("cu_seqlens", cu_seqlens), ("ctx_lens", ctx_lens)):
+            if t is not None:
+                _need_ints(fn, name, t, 1, dev)
+        if cu_seqlens.shape[0] != S + 1:
+            _fail(fn, f"cu_seqlens has {cu_seqlens.shape[0]} entries for {S} sequences")
+        _fail(fn, f"ctx_lens has {ctx_lens.shape[0]} entries for {S} sequences")
     return S
 
 
 def _tables(fn, dev, block_table, ring_table):
-    _ints(fn, "block_table", block_table, dev, 2)
+    """(slots, block pages, ring pages) of the tables."""
+    _need_ints(fn, "block_table", block_table, 2, dev)
     n_slots, nbp = block_table.shape
     if ring_table is None:
         return n_slots, nbp, 0
-    _ints(fn, "ring_table", ring_table, dev, 2)
-    if ring_table.shape[0] != n_slots:
-        _fail(fn, f"ring_table has {ring_table.shape[0]} slots, block_table {n_slots}")
-    return n_slots, nbp, ring_table.shape[1]
+    _need_ints(fn, "ring_table", ring_table, 2, dev)
+    m, nrp = ring_table.shape
+    if m != n_slots:
+        _fail(fn, f"ring_table has {m} slots, block_table {n_slots}")
+    return n_slots, nbp, nrp
 
 
 def _rows2d(x):
     """``x`` ``[N, c]`` with 16-byte aligned rows, and their stride."""
-    es = x.element_size()
-    if x.stride(1) != 1 or (x.stride(0) * es) % 16 or x.data_ptr() % 16 or x.stride(0) < x.shape[1]:
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x, x.stride(0)
+    ld, one = x.stride()
+    if one != 1 or (ld * x.element_size()) % 16 or x.data_ptr() % 16 or ld < x.shape[1]:
+        x = x.detach().clone(memory_format=torch.contiguous_format)
+        ld = x.shape[1]
+    return x, ld
 
 
-def _on(dev):
-    """Makes ``dev`` the current device of a launch where it is not."""
-    return torch.cuda.device(dev)
+def _f32_rows(t, dev):
+    """fp32, contiguous and 16-byte aligned on device ``dev``: ``t`` itself where it is."""
+    if t.dtype is torch.float32 and t.get_device() == dev and t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    return _aligned(_f32_cached(t, torch.device("cuda", dev)))
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
 
 
 def hca_paged_append(C, Z, B_pos, rows, scales, state, block_table, ring_table, slots, cu_seqlens,
@@ -107,34 +124,32 @@ def hca_paged_append(C, Z, B_pos, rows, scales, state, block_table, ring_table, 
     may occur once.
     """
     fn = "hca_paged_append"
-    _lib.require_gpu(fn, C, Z, rows)
-    fmt, P, page, c = _pool(fn, rows, scales)
-    dev = rows.device
-    if C.dim() != 2 or C.shape != Z.shape or C.shape[1] != c or C.dtype != Z.dtype or C.device != dev \
-            or Z.device != dev:
-        _fail(fn, f"C and Z must be [N, {c}] of one dtype on {dev}, got {tuple(C.shape)} {C.dtype} and "
+    if not (C.is_cuda and Z.is_cuda and rows.is_cuda):
+        _lib.require_gpu(fn, C, Z, rows)
+    fmt, P, page, c, dev = _pool(fn, rows, scales)
+    if C.dim() != 2 or C.shape != Z.shape or C.shape[1] != c or C.dtype is not Z.dtype \
+            or C.get_device() != dev or Z.get_device() != dev:
+        _fail(fn, f"C and Z must be [N, {c}] of one dtype on {rows.device}, got {tuple(C.shape)} {C.dtype} and "
                   f"{tuple(Z.shape)} {Z.dtype}")
     if m2 < 1:
         _fail(fn, f"m2={m2} must be >= 1")
     if B_pos.shape != (m2, c):
         _fail(fn, f"B_pos.shape={tuple(B_pos.shape)} must equal (m2, c)=({m2}, {c})")
     n_slots, nbp, nrp = _tables(fn, dev, block_table, ring_table)
-    if state.dtype != torch.float32 or state.shape != (n_slots, 3, c) or not state.is_contiguous() \
-            or state.device != dev:
-        _fail(fn, f"state must be contiguous float32 [{n_slots}, 3, {c}] on {dev}")
+    if state.dtype is not torch.float32 or state.shape != (n_slots, 3, c) or not state.is_contiguous() \
+            or state.get_device() != dev:
+        _fail(fn, f"state must be contiguous float32 [{n_slots}, 3, {c}] on {rows.device}")
     S = _step(fn, dev, slots, cu_seqlens, ctx_lens)
     if max_len < 0 or (nrp and max_len > nrp * page):
         _fail(fn, f"max_len={max_len} must be at most the ring's {nrp * page} rows")
     code = _lib.dtype_code(fn, C.dtype)
-    C, ldc = _rows2d(C.detach())
-    Z, ldz = _rows2d(Z.detach())
-    B_pos = _aligned(_f32_cached(B_pos, dev))
-    ptr = _lib.ptr
-    with _on(dev):
-        _lib.call("kch_hca_paged_append", ptr(C), ldc, ptr(Z), ldz, ptr(B_pos), ptr(rows), ptr(scales),
-                  ptr(state), ptr(block_table), ptr(ring_table), ptr(slots), ptr(cu_seqlens),
-                  ptr(ctx_lens), S, C.shape[0], c, m2, P, page, nbp, nrp, n_slots, max_len,
-                  int(normalize), fmt, code, _lib.stream_of(rows))
+    C, ldc = _rows2d(C)
+    Z, ldz = _rows2d(Z)
+    B_pos = _f32_rows(B_pos, dev)
+    _lib.call_on(dev, "kch_hca_paged_append", C.data_ptr(), ldc, Z.data_ptr(), ldz, B_pos.data_ptr(),
+                 rows.data_ptr(), _p(scales), state.data_ptr(), block_table.data_ptr(), _p(ring_table),
+                 slots.data_ptr(), cu_seqlens.data_ptr(), ctx_lens.data_ptr(), S, C.shape[0], c, m2, P, page,
+                 nbp, nrp, n_slots, max_len, 1 if normalize else 0, fmt, code)
 
 
 def hca_paged_attention(q, rows, scales, block_table, ring_table, slots, cu_seqlens, ctx_lens, *, m2,
@@ -151,11 +166,11 @@ def hca_paged_attention(q, rows, scales, block_table, ring_table, slots, cu_seql
     The products are bf16 with fp32 sums whatever ``q``'s type.
     """
     fn = "hca_paged_attention"
-    _lib.require_gpu(fn, q, rows)
-    fmt, P, page, c = _pool(fn, rows, scales)
-    dev = rows.device
-    if q.dim() != 3 or q.shape[2] != c or q.shape[1] < 1 or q.device != dev:
-        _fail(fn, f"q must be [N, nh, {c}] on {dev}, got {tuple(q.shape)} on {q.device}")
+    if not (q.is_cuda and rows.is_cuda):
+        _lib.require_gpu(fn, q, rows)
+    fmt, P, page, c, dev = _pool(fn, rows, scales)
+    if q.dim() != 3 or q.shape[2] != c or q.shape[1] < 1 or q.get_device() != dev:
+        _fail(fn, f"q must be [N, nh, {c}] on {rows.device}, got {tuple(q.shape)} on {q.device}")
     N, nh, _ = q.shape
     code = _lib.dtype_code(fn, q.dtype)
     if m2 < 1:
@@ -171,27 +186,27 @@ def hca_paged_attention(q, rows, scales, block_table, ring_table, slots, cu_seql
         max_ctx = nbp * page * m2
     if max_ctx < 0:
         _fail(fn, f"max_ctx={max_ctx} must be >= 0")
-    max_ctx = min(max_ctx, 2 ** 31 - 1)
-    sink = None
+    if max_ctx >= 2 ** 31:
+        max_ctx = 2 ** 31 - 1
     if sink_logits is not None:
         if sink_logits.shape != (nh,):
             _fail(fn, f"sink_logits.shape={tuple(sink_logits.shape)} must equal (nh,)=({nh},)")
-        sink = _f32_cached(sink_logits, dev)
-    tail = out is None
-    if tail:
-        out = torch.empty(N, nh, c, device=dev, dtype=q.dtype)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous() \
-            or out.data_ptr() % 16:
-        _fail(fn, f"out must be a contiguous, 16-byte aligned {tuple(q.shape)} {q.dtype} tensor on {dev}")
-    q = _aligned(q.detach())
-    ptr = _lib.ptr
+        sink_logits = _f32_rows(sink_logits, dev)
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = _aligned(q.detach())
+    tail = 0
+    if out is None:
+        tail = 1
+        out = torch.empty(N, nh, c, device=rows.device, dtype=q.dtype)
+    elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != dev \
+            or not out.is_contiguous() or out.data_ptr() % 16:
+        _fail(fn, f"out must be a contiguous, 16-byte aligned {tuple(q.shape)} {q.dtype} tensor on {rows.device}")
     nbytes = _lib.load().kch_hca_paged_attn_ws_bytes(S, N, nh, c, m2, sliding_window, max_len, max_ctx)
-    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
-    with _on(dev):
-        _lib.call("kch_hca_paged_attn", ptr(q), ptr(sink), ptr(out), ptr(rows), ptr(scales),
-                  ptr(block_table), ptr(ring_table), ptr(slots), ptr(cu_seqlens), ptr(ctx_lens), S, N, nh,
-                  c, m2, sliding_window, P, page, nbp, nrp, n_slots, max_len, max_ctx, float(scale),
-                  int(normalize_q), int(tail), fmt, code, ptr(ws), nbytes, _lib.stream_of(rows))
+    ws = torch.empty(nbytes, device=rows.device, dtype=torch.uint8) if nbytes else None
+    _lib.call_on(dev, "kch_hca_paged_attn", q.data_ptr(), _p(sink_logits), out.data_ptr(), rows.data_ptr(),
+                 _p(scales), block_table.data_ptr(), _p(ring_table), slots.data_ptr(), cu_seqlens.data_ptr(),
+                 ctx_lens.data_ptr(), S, N, nh, c, m2, sliding_window, P, page, nbp, nrp, n_slots, max_len,
+                 max_ctx, scale, 1 if normalize_q else 0, tail, fmt, code, _p(ws), nbytes)
     return out
 
 
@@ -201,24 +216,24 @@ def paged_read(rows, scales, table, slots, cu_rows, *, total, first=None, dtype=
     table), capacity its pages times their rows. ``total`` is the number of result rows; those
     behind the last sequence are zeros (in ``out`` as they were)."""
     fn = "paged_read"
-    _lib.require_gpu(fn, rows)
-    fmt, P, page, c = _pool(fn, rows, scales)
-    dev = rows.device
-    _ints(fn, "table", table, dev, 2)
+    if not rows.is_cuda:
+        _lib.require_gpu(fn, rows)
+    fmt, P, page, c, dev = _pool(fn, rows, scales)
+    _need_ints(fn, "table", table, 2, dev)
     S = _step(fn, dev, slots, cu_rows, first)
     if total < 0:
         _fail(fn, f"total={total} must be >= 0")
-    tail = out is None
-    if tail:
-        out = torch.empty(total, c, device=dev, dtype=dtype)
-    elif out.shape != (total, c) or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
-        _fail(fn, f"out must be a contiguous, 16-byte aligned [{total}, {c}] tensor on {dev}")
+    tail = 0
+    if out is None:
+        tail = 1
+        out = torch.empty(total, c, device=rows.device, dtype=dtype)
+    elif out.shape != (total, c) or out.get_device() != dev or not out.is_contiguous() or out.data_ptr() % 16:
+        _fail(fn, f"out must be a contiguous, 16-byte aligned [{total}, {c}] tensor on {rows.device}")
     code = _lib.dtype_code(fn, out.dtype)
-    ptr = _lib.ptr
-    with _on(dev):
-        _lib.call("kch_paged_read", ptr(rows), ptr(scales), ptr(table), ptr(slots), ptr(cu_rows), ptr(first),
-                  ptr(out), S, total, c, P, page, table.shape[1], table.shape[0], int(tail), fmt, code,
-                  _lib.stream_of(rows))
+    n_slots, nbp = table.shape
+    _lib.call_on(dev, "kch_paged_read", rows.data_ptr(), _p(scales), table.data_ptr(), slots.data_ptr(),
+                 cu_rows.data_ptr(), _p(first), out.data_ptr(), S, total, c, P, page, nbp, n_slots, tail, fmt,
+                 code)
     return out
 
 
