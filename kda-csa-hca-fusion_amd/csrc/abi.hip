@@ -1564,7 +1564,8 @@ static int paged_pool(const char* fn, kch::PagedPool& pl, const void* rows, cons
   if (S > 0 && N > 0) {
     if (!slots || !cu || (n_slots > 0 && ((nbp > 0 && !block_table) || (nrp > 0 && !ring_table))))
       return fail(KCH_ERR_INVALID, "%s: null table pointer", fn);
-    if (P > 0 && (!rows || (format != 0 && !scales))) return fail(KCH_ERR_INVALID, "%s: null pool pointer", fn);
+    if (P < 1) return fail(KCH_ERR_INVALID, "%s: a pool without pages", fn);
+    if (!rows || (format != 0 && !scales)) return fail(KCH_ERR_INVALID, "%s: null pool pointer", fn);
     if ((uintptr_t)rows & 15) return fail(KCH_ERR_INVALID, "%s: rows must be 16-byte aligned", fn);
   }
   pl.rows = const_cast<void*>(rows);
@@ -1644,8 +1645,8 @@ int kch_hca_paged_attn(const void* q, const float* sink, void* out, const void* 
   p.part_o = static_cast<float*>(ws);
   p.part_ml = p.part_o ? p.part_o + (size_t)pl.nsplit * N * nh * c : nullptr;
   p.nh = nh; p.m2 = m2; p.win = win; p.max_len = max_len; p.normalize_q = normalize_q;
-  p.zero_tail = zero_tail; p.nsplit = pl.nsplit; p.split_keys = pl.split_keys; p.scale = scale;
-  return hip_status(fn, kch::paged_attn_dispatch(p, pl, format, dtype, (hipStream_t)stream));
+  p.zero_tail = zero_tail; p.rows = pl.rows; p.nsplit = pl.nsplit; p.range = pl.range; p.scale = scale;
+  return hip_status(fn, kch::paged_attn_dispatch(p, format, dtype, (hipStream_t)stream));
 }
 
 int kch_paged_read(const void* rows, const void* scales, const int* table, const int* slots, const int* cu,

@@ -464,18 +464,20 @@ struct PagedAttnParams {
   void* out;              // [N, nh, c]
   float* part_o;          // [nsplit, N nh, c] partial outputs (nsplit > 1)
   float* part_ml;         // [nsplit, N nh, 2] their softmax reference and sum
-  int nh, m2, win, max_len, normalize_q, zero_tail, nsplit, split_keys;
+  int nh, m2, win, max_len, normalize_q, zero_tail;
+  int rows, nsplit, range;  // the plan's
   float scale;
 };
-// How a call is laid out: query rows of a workgroup, key ranges and their length,
-// and the workspace that the ranges need.
+// How a call is laid out: query rows of a workgroup (up to kPagedTokenRows of them the
+// waves split the keys), ranges of keys and their length (in keys, or in 32-key
+// steps where the waves split them), and the workspace that the ranges need.
+constexpr int kPagedTokenRows = 32;
 struct PagedAttnPlan {
-  int rows, nsplit, split_keys;
+  int rows, nsplit, range;
   size_t bytes;
 };
 PagedAttnPlan paged_attn_plan(int S, int N, int nh, int c, int m2, int win, int max_len, int max_ctx);
-hipError_t paged_attn_dispatch(const PagedAttnParams& p, const PagedAttnPlan& plan, int format, int dtype,
-                               hipStream_t s);
+hipError_t paged_attn_dispatch(const PagedAttnParams& p, int format, int dtype, hipStream_t s);
 
 // Few rows times 4-bit weights (linear_w4.hip): y [M, N] = x [M, K] W^T (+ res), W[n, k] =
 // scales[k / group][n] (code - zeros[k / group][n]), codes [N, K / 2] two a byte.

@@ -15,11 +15,14 @@
 // several tokens: each lane masks its own row. A workgroup takes RG groups of
 // 16 rows and streams the union of their keys through LDS, KC rows at a time:
 // page entries two tiles ahead, rows one tile ahead in registers, converted to
-// bf16 once on their way into LDS for all of the workgroup's rows. Where a step
-// has few rows (one token of 16 heads is one group) the workgroup's waves split
-// each tile's keys instead (KG waves a group) and their sums are joined at the
-// end; long contexts are cut into ranges of keys, one workgroup each, whose
-// partial sums a second kernel joins, so that a few sequences fill the device.
+// bf16 once on their way into LDS for all of the workgroup's rows
+// (paged_attn_kernel). Where a sequence has few rows (one token of 16 heads is one
+// group) the call is bound by the rows' bytes, and the waves of a workgroup split
+// the keys: each takes 32-key steps of its own through its own LDS, two of them in
+// flight, without a barrier, and the waves' sums are joined at the end
+// (paged_token_kernel). Long contexts are cut into ranges of keys, one workgroup
+// each, whose partial sums a second kernel joins, so that a few sequences fill the
+// device.
 //
 // A key row that is not finite (E8M0 code 255, or a non-finite bf16 channel)
 // sits in LDS as zeros beside a NaN that is added to its scores: rows that do
@@ -32,7 +35,8 @@ namespace kch {
 
 namespace {
 
-constexpr int KC = 128;  // key rows of an LDS tile
+constexpr int KC = 128;       // key rows of an LDS tile
+constexpr int kStepUnit = 8;  // 32-key steps of a range: two a wave
 
 // The keys of query tokens [ta, tb] (indices into the chunk) of a sequence: the
 // first nc compressed rows, then nw window rows from position wlo on.
@@ -50,315 +54,629 @@ __device__ __forceinline__ KeySpan key_span(const PagedAttnParams& p, const Page
   k.nw = p.win > 0 && p.pool.nrp > 0 ? pb - k.wlo + 1 : 0;
   return k;
 }
-// Keys of one range: split_keys, or more where the spans are longer than the
-// launch was laid out for.
-__device__ __forceinline__ uint32_t range_keys(const PagedAttnParams& p, uint32_t total) {
+// The same keys as 32-key steps of paged_token_kernel: nb steps of compressed
+// rows, then nw of window rows. Where pages hold whole steps (at least 32 rows) a
+// step never leaves its page: window steps then start at a multiple of 32 of the
+// ring, woff rows before the first one.
+struct KeySteps {
+  uint32_t nb, nw, woff;
+};
+__device__ __forceinline__ KeySteps key_steps(const PagedAttnParams& p, const KeySpan& sp) {
+  KeySteps k;
+  k.nb = (sp.nc + 31) / 32;
+  const uint32_t cap = (uint32_t)p.pool.nrp << p.pool.log2page;
+  k.woff = sp.nw && p.pool.log2page >= 5 ? (sp.wlo % cap) & 31 : 0;
+  k.nw = sp.nw ? (k.woff + sp.nw + 31) / 32 : 0;
+  return k;
+}
+// Length of a range, in units of the kernel that takes it: the plan's, or more where
+// the spans are longer than the launch was laid out for.
+__device__ __forceinline__ uint32_t range_len(const PagedAttnParams& p, uint32_t total, uint32_t unit) {
   const uint32_t need = (total + p.nsplit - 1) / p.nsplit;
-  return max((uint32_t)p.split_keys, (need + KC - 1) / KC * KC);
+  return max((uint32_t)p.range, (need + unit - 1) / unit * unit);
 }
 
-// RG groups of 16 rows, QW of them a wave, KG waves share a group's keys.
-template <int HD, int FMT, int RG, int QW, int KG, typename T>
-__global__ __launch_bounds__(64 * (RG / QW) * KG) void paged_attn_kernel(PagedAttnParams p) {
+// Output rows n0 .. n1 - 1 as zeros, by the workgroup.
+template <int HD, typename T>
+__device__ __forceinline__ void zero_rows(const PagedAttnParams& p, long long n0, long long n1) {
+  for (long long i = n0 * HD + 4ll * threadIdx.x; i < n1 * HD; i += 4ll * blockDim.x)
+    Store4<T>::run(static_cast<T*>(p.out) + i, f32x4{0.f, 0.f, 0.f, 0.f}, 1.f);
+}
+// The rows that no workgroup computes: those behind the last sequence (a share of each
+// workgroup of a grid row of their own), and what a chunk has past max_len.
+template <int HD, typename T>
+__device__ __forceinline__ void zero_tail(const PagedAttnParams& p) {
+  if (blockIdx.z) return;
+  const long long r0 = (long long)max(0, min(p.pool.cu[p.pool.S], p.pool.N)) * p.nh, r1 = (long long)p.pool.N * p.nh;
+  const long long per = (r1 - r0 + gridDim.x - 1) / gridDim.x, at = r0 + per * blockIdx.x;
+  zero_rows<HD, T>(p, at, min(r1, at + per));
+}
+__device__ __forceinline__ int computed_rows(const PagedAttnParams& p, const PagedSeq& sq) {
+  return min(sq.len, p.max_len) * p.nh;  // N nh is below 2^30
+}
+
+// One 16-row group's output, or its partial sums for the join of its ranges.
+template <int HD, typename T>
+__device__ __forceinline__ void store_group(const PagedAttnParams& p, const MqaWave<HD>& w, long long g, int live,
+                                            bool whole, int head, void* stage) {
+  if (whole) {
+    const float f = w.finish(p.sink != nullptr, p.sink ? p.sink[head] : 0.f);
+    store_rows<HD, T>(w.o, f, static_cast<T*>(p.out) + g * HD, live, stage);
+    return;
+  }
+  const int n = lane_id() & 15;
+  const long long gp = (long long)blockIdx.z * p.pool.N * p.nh + g;
+  store_rows<HD, float>(w.o, 1.f, p.part_o + gp * HD, live, stage);
+  if (lane_id() < 16 && n < live) {
+    p.part_ml[2 * (gp + n)] = w.M;
+    p.part_ml[2 * (gp + n) + 1] = w.L;
+  }
+}
+
+// Up to 16 QW rows of a sequence and a range of 32-key steps, which the four waves take
+// in turn. BIG: pages of at least 32 rows (one table entry a step). No load is behind a
+// branch (a wait there would drain every load in flight): past the end the last
+// step is read again.
+// Workgroups a CU at least (what keeps two steps in registers without spilling).
+constexpr int token_min_blocks(int HD, int FMT, int QW) {
+  return (QW == 1 ? 3 : 2) - (HD == 128 && FMT == PF_BF16 ? 1 : 0);
+}
+template <int HD, int FMT, int QW, bool BIG, typename T>
+__global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_token_kernel(PagedAttnParams p) {
   using W = MqaWave<HD>;
-  constexpr int NWV = RG / QW * KG, NTH = 64 * NWV;
+  constexpr int ROWB = FMT == PF_BF16 ? 2 * HD : HD;  // bytes of a key row
+  constexpr int TPR = ROWB / 16;                      // lanes per key row
+  constexpr int RPI = 64 / TPR;                       // key rows of a load
+  constexpr int NLI = 32 / RPI;                       // loads of a step
+  constexpr int NP = BIG ? 1 : NLI;                   // table entries of a lane
+  __shared__ __attribute__((aligned(16))) bf16_t stage_all[4][32 * HD];
+  __shared__ float ml[4][16][2];
+  __shared__ float poison[4][32];
+  const PagedPool& pl = p.pool;
+  if (blockIdx.y == (unsigned)pl.S) return zero_tail<HD, T>(p);
+  const PagedSeq sq = paged_seq(pl, blockIdx.y);
+  const int nrow = computed_rows(p, sq);
+  if (p.zero_tail && sq.len > p.max_len && !(blockIdx.x | blockIdx.z))
+    zero_rows<HD, T>(p, (long long)sq.row0 * p.nh + nrow, (long long)(sq.row0 + sq.len) * p.nh);
+  const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int lane = lane_id(), q4 = lane >> 4, n = lane & 15;
+  const int lrow = lane / TPR, lch = lane % TPR;
+  const uint32_t cap = (uint32_t)pl.nrp << pl.log2page;
+  const uint32_t lmask = (1u << pl.log2page) - 1;
+  bf16_t* const stage = stage_all[wv];
+  const TileOffsets<HD> to;
+
+  const int r0 = blockIdx.x * 16 * QW;
+  if (r0 >= nrow) return;
+  const KeySpan sp = key_span(p, sq, r0 / p.nh, (min(r0 + 16 * QW, nrow) - 1) / p.nh);
+  const KeySteps ks = key_steps(p, sp);
+  const uint32_t total = ks.nb + ks.nw, per = range_len(p, total, kStepUnit);
+  const uint32_t s0 = per * blockIdx.z, s1 = min(total, s0 + per);
+  if (s0 >= total && blockIdx.z) return;
+  const bool whole = total <= per;  // no other range: the output itself
+  const int* const btab = pl.block_table + (size_t)sq.slot * pl.nbp;
+  const int* const rtab = pl.ring_table + (size_t)sq.slot * pl.nrp;
+  const uint32_t wr = sp.nw ? sp.wlo % cap - ks.woff : 0;  // ring row of the first window step
+
+  W w[QW];
+  int head[QW];
+  if (s0 < s1) {
+    const int nb = ks.nb, last = s1 - 1;
+    const uint32_t bwidth = pl.nbp, rwidth = pl.nrp;
+    struct Step {
+      uint4 v[NLI];
+      int code[NLI];
+      int ok;  // bit i: the row of load i is a row of the pool
+    };
+    auto step_row = [&](int i) { return (uint32_t)(RPI * i + lrow); };
+    auto ring_row = [&](uint32_t r) { return r >= cap ? r - cap : r; };
+    auto load_page = [&](int st, int (&pg)[NP]) {
+      st = min(st, last);
+      const int d = st - nb;  // (a signed compare stays on the scalar unit)
+      const bool blk = d < 0;
+      const int* const tab = blk ? btab : rtab;
+      const uint32_t f = blk ? 32 * st : wr + 32 * d, width = blk ? bwidth : rwidth;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        uint32_t r = BIG ? f : f + step_row(i);
+        if (!blk) r = ring_row(r);
+        pg[i] = tab[min(r >> pl.log2page, width - 1)];
+      }
+    };
+    auto load_step = [&](int st, const int (&pg)[NP], Step& s) {
+      st = min(st, last);
+      const int d = st - nb;
+      const bool blk = d < 0;
+      const uint32_t f = blk ? 32 * st : wr + 32 * d;
+      if constexpr (BIG) {  // one page: a scalar address, the lane's offset in it and constants
+        const int page = __builtin_amdgcn_readfirstlane(pg[0]);
+        const bool ok = (unsigned)page < (unsigned)pl.P;
+        const long long pr = ((long long)(ok ? page : 0) << pl.log2page) + ((blk ? f : ring_row(f)) & lmask);
+        const char* const base = static_cast<const char*>(pl.rows) + pr * ROWB;
+        const uint8_t* const sb = pl.scales + pr;
+#pragma unroll
+        for (int i = 0; i < NLI; ++i) {
+          s.v[i] = *reinterpret_cast<const uint4*>(base + (lrow * ROWB + 16 * lch) + i * RPI * ROWB);
+          if constexpr (FMT != PF_BF16) s.code[i] = sb[lrow + i * RPI];
+        }
+        s.ok = ok ? 0xff : 0;
+      } else {
+        s.ok = 0;
+#pragma unroll
+        for (int i = 0; i < NLI; ++i) {
+          const bool ok = (unsigned)pg[i] < (unsigned)pl.P;
+          uint32_t r = f + step_row(i);
+          if (!blk) r = ring_row(r);
+          const long long pr = ((long long)(ok ? pg[i] : 0) << pl.log2page) + (r & lmask);
+          s.v[i] = *reinterpret_cast<const uint4*>(static_cast<const char*>(pl.rows) + pr * ROWB + 16 * lch);
+          if constexpr (FMT != PF_BF16) s.code[i] = pl.scales[pr];
+          s.ok |= (ok ? 1 : 0) << i;
+        }
+      }
+    };
+    // two steps in flight, and the table entries of the two after them. The loads keep
+    // this order everywhere: a wait counts the loads issued after the one it waits for.
+    int pa[NP], pb[NP];
+    Step sa, sb;
+    int st = s0 + wv;
+    auto next = [&](int at, int (&pg)[NP], Step& s) {
+      __builtin_amdgcn_sched_barrier(0);
+      load_step(at, pg, s);
+      __builtin_amdgcn_sched_barrier(0);
+      load_page(at + 8, pg);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    load_page(st, pa);
+    __builtin_amdgcn_sched_barrier(0);
+    load_page(st + 4, pb);
+    next(st, pa, sa);
+    next(st + 4, pb, sb);
+
+    // the queries, while the first steps' rows are in flight; this lane's row sees
+    // block rows below vis, and window rows [lo, hi) counted from the first window step's
+    uint32_t vis[QW], lo[QW], hi[QW];
+#pragma unroll
+    for (int u = 0; u < QW; ++u) {
+      const int r = r0 + 16 * u + n;
+      const bool live = r < nrow;
+      const int rr = live ? r : nrow - 1;
+      const int tok = rr / p.nh;
+      head[u] = rr - tok * p.nh;
+      w[u].template init_always<T>(static_cast<const T*>(p.q) + ((long long)sq.row0 * p.nh + rr) * HD, live,
+                                   p.normalize_q != 0, p.scale);
+      const uint32_t pos = sq.ctx + tok;
+      const uint32_t f = pos + 1 > (uint32_t)p.win ? pos + 1 - p.win : 0;
+      // (a padding row is never stored: it masks nothing)
+      vis[u] = live ? visible_blocks(p, pos) : 0xffffffffu;
+      lo[u] = live ? ks.woff + (f - sp.wlo) : 0;
+      hi[u] = live ? ks.woff + (pos - sp.wlo) + 1 : 0xffffffffu;
+    }
+
+    bool any_bad = false;
+    // a step's rows into the wave's LDS
+    auto put = [&](int st, Step& s) {
+      const int d = st - nb;
+      const bool blk = d < 0;
+      const uint32_t j0 = 32 * (blk ? st : d);  // block row, or window row, of the step's first
+      // rows that no query of the workgroup sees, or that are none of the pool: zeros
+      const uint32_t ua = blk ? 0 : ks.woff, ub = st > last ? 0 : blk ? sp.nc : ks.woff + sp.nw;
+      if (!(BIG && s.ok && j0 >= ua && j0 + 32 <= ub)) {
+#pragma unroll
+        for (int i = 0; i < NLI; ++i) {
+          const uint32_t j = j0 + step_row(i);
+          const bool ok = (s.ok >> i & 1) && j >= ua && j < ub;
+          s.v[i] = ok ? s.v[i] : make_uint4(0, 0, 0, 0);
+          if constexpr (FMT != PF_BF16) s.code[i] = ok ? s.code[i] : 127;
+        }
+      }
+      bool bad[NLI], some = false;
+#pragma unroll
+      for (int i = 0; i < NLI; ++i) {
+        if constexpr (FMT == PF_BF16) {
+          const uint32_t x[4] = {s.v[i].x, s.v[i].y, s.v[i].z, s.v[i].w};
+          bad[i] = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) bad[i] |= (x[e] & 0x7f80u) == 0x7f80u || (x[e] & 0x7f800000u) == 0x7f800000u;
+        } else {
+          bad[i] = s.code[i] == kScaleNan;
+        }
+        some |= bad[i];
+      }
+      wave_lds_sync();  // the previous step's reads of the stage are done
+      any_bad = __ballot(some) != 0ull;
+      if (any_bad) {  // (rare) such a row as zeros, and NaN beside it
+#pragma unroll
+        for (int i = 0; i < NLI; ++i) {
+          const unsigned long long g = __ballot(bad[i]) >> (lane & ~(TPR - 1)) & ((1ull << TPR) - 1);
+          s.v[i] = g ? make_uint4(0, 0, 0, 0) : s.v[i];
+          if constexpr (FMT != PF_BF16) s.code[i] = g ? 127 : s.code[i];
+          if (lch == 0) poison[wv][step_row(i)] = g ? __uint_as_float(0x7fc00000u) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NLI; ++i) {
+        const uint32_t row = step_row(i);
+        bf16_t* const dst = stage + row * HD;
+        const int sw = tile_swz<HD>(row & 15);
+        if constexpr (FMT == PF_BF16) {
+          *reinterpret_cast<uint4*>(dst + 8 * (lch ^ sw)) = s.v[i];
+        } else {
+          const float sc = __uint_as_float((uint32_t)s.code[i] << 23);
+          const uint2 a = dequant4_bf16<FMT>(s.v[i].x, sc), c = dequant4_bf16<FMT>(s.v[i].y, sc);
+          const uint2 d = dequant4_bf16<FMT>(s.v[i].z, sc), e = dequant4_bf16<FMT>(s.v[i].w, sc);
+          *reinterpret_cast<uint4*>(dst + 8 * ((2 * lch) ^ sw)) = make_uint4(a.x, a.y, c.x, c.y);
+          *reinterpret_cast<uint4*>(dst + 8 * ((2 * lch + 1) ^ sw)) = make_uint4(d.x, d.y, e.x, e.y);
+        }
+      }
+      wave_lds_sync();  // staged rows visible to the whole wave
+    };
+    auto use = [&](int st) {
+      const int d = st - nb;
+      const bool blk = d < 0;
+      const uint32_t j0 = 32 * (blk ? st : d);
+      f32x4 ra[QW], rb[QW];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        bf16x8 kf[W::NS];
+#pragma unroll
+        for (int e = 0; e < W::NS; ++e) kf[e] = *reinterpret_cast<const bf16x8*>(stage + 16 * HD * h + to.key(e));
+#pragma unroll
+        for (int u = 0; u < QW; ++u) {
+          if (h == 0) ra[u] = w[u].scores(kf);
+          else rb[u] = w[u].scores(kf);
+        }
+      }
+      bf16x8 pb8[QW];
+#pragma unroll
+      for (int u = 0; u < QW; ++u) {
+        float sc[8] = {ra[u][0], ra[u][1], ra[u][2], ra[u][3], rb[u][0], rb[u][1], rb[u][2], rb[u][3]};
+        if (any_bad) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sc[e] += poison[wv][4 * q4 + (e < 4 ? e : 12 + e)];
+        }
+        const uint32_t la = blk ? 0 : lo[u], lb = st > last ? 0 : blk ? vis[u] : hi[u];
+        if (__ballot(j0 < la || j0 + 32 > lb)) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t j = j0 + 4 * q4 + (e < 4 ? e : 12 + e);
+            sc[e] = j >= la && j < lb ? sc[e] : -INFINITY;
+          }
+        }
+        pb8[u] = w[u].softmax32(sc);
+      }
+#pragma unroll
+      for (int t = 0; t < W::NT; ++t) {
+        const bf16x8 va = W::vt_frag(stage, to, t);
+#pragma unroll
+        for (int u = 0; u < QW; ++u)
+          w[u].o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb8[u], w[u].o[t], 0, 0, 0);
+      }
+    };
+
+    // A step's registers are free once it is in LDS: the load of the one after the next
+    // goes out before the products. Steps go in pairs, the second one past the range
+    // as one without keys (an exit between them would have the loop's first wait drain
+    // every load).
+    for (; st <= last; st += 8) {
+      put(st, sa);
+      next(st + 8, pa, sa);
+      use(st);
+      put(st + 4, sb);
+      next(st + 12, pb, sb);
+      use(st + 4);
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < QW; ++u) {
+      float z[W::NS][8] = {};
+      w[u].setup(z, false, 1.f);
+      head[u] = 0;
+    }
+  }
+
+  // the four waves' sums, a 16-row group at a time
+#pragma unroll
+  for (int u = 0; u < QW; ++u) {
+    w[u].finalize();
+    float* const ob = reinterpret_cast<float*>(stage_all) + wv * 16 * HD;
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < W::NT; ++t) *reinterpret_cast<f32x4*>(ob + (t * 64 + lane) * 4) = w[u].o[t];
+    if (q4 == 0) {
+      ml[wv][n][0] = w[u].M;
+      ml[wv][n][1] = w[u].L;
+    }
+    __syncthreads();
+    if (wv == u % 4) {
+      float M = ml[0][n][0];
+#pragma unroll
+      for (int g = 1; g < 4; ++g) M = fmaxf(M, ml[g][n][0]);
+      w[u].M = M;
+      w[u].L = 0.f;
+#pragma unroll
+      for (int t = 0; t < W::NT; ++t) w[u].o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float f = fast_exp2(ml[g][n][0] - M);
+        w[u].L += f * ml[g][n][1];
+        const float* og = reinterpret_cast<const float*>(stage_all) + g * 16 * HD;
+#pragma unroll
+        for (int t = 0; t < W::NT; ++t) w[u].o[t] += f * *reinterpret_cast<const f32x4*>(og + (t * 64 + lane) * 4);
+      }
+    }
+    __syncthreads();  // the sums are read before their place is staged over
+    const int r = r0 + 16 * u;
+    if (wv == u % 4 && r < nrow)
+      store_group<HD, T>(p, w[u], (long long)sq.row0 * p.nh + r, min(16, nrow - r), whole, head[u], ob);
+  }
+}
+
+// RG groups of 16 rows of a sequence, QW of them a wave, and a range of keys.
+template <int HD, int FMT, int RG, int QW, typename T>
+__global__ __launch_bounds__(64 * (RG / QW)) void paged_attn_kernel(PagedAttnParams p) {
+  using W = MqaWave<HD>;
+  constexpr int NWV = RG / QW, NTH = 64 * NWV;
   constexpr int ROWS = 16 * RG;
   constexpr int EPL = FMT == PF_BF16 ? 8 : 16;  // row elements of a lane's 16 bytes
   constexpr int TPR = HD / EPL;                 // lanes per key row
   constexpr int RSTEP = NTH / TPR;              // key rows of a load instruction of the workgroup
   constexpr int NLD = KC / RSTEP;
   static_assert(NLD >= 1 && KC % RSTEP == 0 && RSTEP % 16 == 0, "tile loads");
-  static_assert(KG <= KC / 32, "a wave takes whole 32-key steps");
   __shared__ __attribute__((aligned(16))) bf16_t tile[2][KC * HD];
   __shared__ __attribute__((aligned(16))) float poison[2][KC];
   __shared__ int any_bad;  // some row so far is not finite
-  __shared__ float join_ml[KG > 1 ? NWV : 1][16][2];
 
   const int tid = threadIdx.x;
   const PagedPool& pl = p.pool;
-  if (blockIdx.y == (unsigned)pl.S) {  // the rows behind the last sequence
-    if (blockIdx.z) return;
-    const long long n0 = (long long)max(0, min(pl.cu[pl.S], pl.N)) * p.nh * HD, n1 = (long long)pl.N * p.nh * HD;
-    for (long long i = n0 + 8ll * (blockIdx.x * NTH + tid); i < n1; i += 8ll * gridDim.x * NTH)
-#pragma unroll
-      for (int e = 0; e < 8; e += 4) Store4<T>::run(static_cast<T*>(p.out) + i + e, f32x4{0.f, 0.f, 0.f, 0.f}, 1.f);
-    return;
-  }
+  if (blockIdx.y == (unsigned)pl.S) return zero_tail<HD, T>(p);
   const PagedSeq sq = paged_seq(pl, blockIdx.y);
-  const int nrow = sq.len * p.nh;  // N nh is below 2^31
+  const int nrow = computed_rows(p, sq);
+  if (p.zero_tail && sq.len > p.max_len && !(blockIdx.x | blockIdx.z))
+    zero_rows<HD, T>(p, (long long)sq.row0 * p.nh + nrow, (long long)(sq.row0 + sq.len) * p.nh);
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, q4 = lane >> 4, n = lane & 15;
-  const int rg = wv / KG, kg = wv % KG;
   const uint32_t ring_cap = (uint32_t)pl.nrp << pl.log2page;
   const int lmask = (1 << pl.log2page) - 1;
   const int* const btab = pl.block_table + (size_t)sq.slot * pl.nbp;
   const int* const rtab = pl.ring_table + (size_t)sq.slot * pl.nrp;
   const TileOffsets<HD> to;
 
-  // (r0 + the grid's rows cannot pass 2^31: both are at most N nh plus a tile)
-  for (int r0 = blockIdx.x * ROWS; r0 < nrow; r0 += gridDim.x * ROWS) {
-    const int ta = r0 / p.nh, tb = (min(r0 + ROWS, nrow) - 1) / p.nh;
-    const KeySpan sp = key_span(p, sq, ta, tb);
-    const uint32_t total = sp.nc + sp.nw;
-    const uint32_t per = range_keys(p, total);
-    const uint32_t k0 = per * blockIdx.z;
-    if (k0 >= total && blockIdx.z) continue;
-    const uint32_t k1 = min(total, k0 + per);
-    const bool whole = total <= per;  // no other range: the output itself
+  const int r0 = blockIdx.x * ROWS;
+  if (r0 >= nrow) return;
+  const int ta = r0 / p.nh, tb = (min(r0 + ROWS, nrow) - 1) / p.nh;
+  const KeySpan sp = key_span(p, sq, ta, tb);
+  const uint32_t total = sp.nc + sp.nw;
+  const uint32_t per = range_len(p, total, KC);
+  const uint32_t k0 = per * blockIdx.z;
+  if (k0 >= total && blockIdx.z) return;
+  const uint32_t k1 = min(total, k0 + per);
+  const bool whole = total <= per;  // no other range: the output itself
 
-    // Tile loads: thread tid takes 16 bytes (part tid % TPR) of key rows
-    // tid / TPR + RSTEP i of the tile. Rows past k1, and rows whose table entry
-    // names no page of the pool, are zeros.
-    const int lrow = tid / TPR, lch = tid % TPR;
-    const uint32_t wr = sp.nw ? sp.wlo % ring_cap : 0;
-    int pg[NLD];
-    uint4 pf[NLD];
-    int code[NLD];
-    auto line_of = [&](uint32_t j, bool& blk) -> uint32_t {
-      blk = j < sp.nc;
-      if (blk) return j;
-      uint32_t r = wr + (j - sp.nc);
-      return r >= ring_cap ? r % ring_cap : r;
-    };
-    auto load_pages = [&](uint32_t t0) {
+  // Tile loads: thread tid takes 16 bytes (part tid % TPR) of key rows
+  // tid / TPR + RSTEP i of the tile. Rows past k1, and rows whose table entry
+  // names no page of the pool, are zeros.
+  const int lrow = tid / TPR, lch = tid % TPR;
+  const uint32_t wr = sp.nw ? sp.wlo % ring_cap : 0;
+  int pg[NLD];
+  uint4 pf[NLD];
+  int code[NLD];
+  auto line_of = [&](uint32_t j, bool& blk) -> uint32_t {
+    blk = j < sp.nc;
+    if (blk) return j;
+    uint32_t r = wr + (j - sp.nc);
+    return r >= ring_cap ? r % ring_cap : r;
+  };
+  auto load_pages = [&](uint32_t t0) {
 #pragma unroll
-      for (int i = 0; i < NLD; ++i) {
-        const uint32_t j = t0 + lrow + RSTEP * i;
-        pg[i] = -1;
-        if (j < k1) {
-          bool blk;
-          const uint32_t r = line_of(j, blk);
-          pg[i] = (blk ? btab : rtab)[r >> pl.log2page];
-        }
-      }
-    };
-    auto load_rows = [&](uint32_t t0) {
-#pragma unroll
-      for (int i = 0; i < NLD; ++i) {
-        const uint32_t j = t0 + lrow + RSTEP * i;
+    for (int i = 0; i < NLD; ++i) {
+      const uint32_t j = t0 + lrow + RSTEP * i;
+      pg[i] = -1;
+      if (j < k1) {
         bool blk;
         const uint32_t r = line_of(j, blk);
-        const bool ok = (unsigned)pg[i] < (unsigned)pl.P;
-        const long long pr = ok ? ((long long)pg[i] << pl.log2page) + (r & lmask) : 0;
-        pf[i] = make_uint4(0, 0, 0, 0);
-        code[i] = 127;
-        if (ok) {
-          pf[i] = *reinterpret_cast<const uint4*>(static_cast<const char*>(pl.rows) +
-                                                  (pr * TPR + lch) * 16);
-          if constexpr (FMT != PF_BF16) code[i] = pl.scales[pr];
-        }
-      }
-    };
-    auto store_rows_lds = [&](int buf) {
-      bool bad_any = false;
-#pragma unroll
-      for (int i = 0; i < NLD; ++i) {
-        const int row = lrow + RSTEP * i;
-        bf16_t* dst = tile[buf] + row * HD;
-        const int sw = tile_swz<HD>(row & 15);
-        if constexpr (FMT == PF_BF16) {
-          const uint32_t w[4] = {pf[i].x, pf[i].y, pf[i].z, pf[i].w};
-          bool bad = false;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            bad |= (w[e] & 0x7f80u) == 0x7f80u || (w[e] & 0x7f800000u) == 0x7f800000u;
-          // the whole row is bad where one of its lanes is
-          const unsigned long long g = __ballot(bad) >> (lane & ~(TPR - 1)) & ((1ull << TPR) - 1);
-          if (g) pf[i] = make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(dst + 8 * (lch ^ sw)) = pf[i];
-          if (lch == 0) poison[buf][row] = g ? __uint_as_float(0x7fc00000u) : 0.f;
-          bad_any |= g != 0;
-        } else {
-          const bool bad = code[i] == kScaleNan;
-          const float sc = row_scale(bad ? 127 : code[i]);
-          const uint32_t keep = bad ? 0u : 0xffffffffu;
-          const uint2 a = dequant4_bf16<FMT>(pf[i].x & keep, sc), b = dequant4_bf16<FMT>(pf[i].y & keep, sc);
-          const uint2 c = dequant4_bf16<FMT>(pf[i].z & keep, sc), d = dequant4_bf16<FMT>(pf[i].w & keep, sc);
-          *reinterpret_cast<uint4*>(dst + 8 * ((2 * lch) ^ sw)) = make_uint4(a.x, a.y, b.x, b.y);
-          *reinterpret_cast<uint4*>(dst + 8 * ((2 * lch + 1) ^ sw)) = make_uint4(c.x, c.y, d.x, d.y);
-          if (lch == 0) poison[buf][row] = bad ? __uint_as_float(0x7fc00000u) : 0.f;
-          bad_any |= bad;
-        }
-      }
-      if (bad_any) any_bad = 1;
-    };
-
-    // the first tile's rows are in flight while the queries load
-    const uint32_t nt = (k1 - min(k0, k1) + KC - 1) / KC;
-    if (nt) {
-      load_pages(k0);
-      load_rows(k0);
-      load_pages(k0 + KC);
-    }
-
-    W w[QW];
-    uint32_t vis[QW], lo[QW], hi[QW];  // this lane's row: keys [0, vis) and [lo, hi)
-    int head[QW];
-#pragma unroll
-    for (int u = 0; u < QW; ++u) {
-      const int r = r0 + 16 * (QW * rg + u) + n;
-      const bool live = r < nrow;
-      const int rr = live ? r : nrow - 1;
-      const int tok = rr / p.nh;
-      head[u] = rr - tok * p.nh;
-      const T* qrow = static_cast<const T*>(p.q) + ((long long)sq.row0 * p.nh + rr) * HD;
-      w[u].template init_always<T>(qrow, live, p.normalize_q != 0, p.scale);
-      const uint32_t pos = sq.ctx + tok;
-      vis[u] = live ? visible_blocks(p, pos) : 0;
-      lo[u] = hi[u] = 0;
-      if (live && sp.nw) {
-        const uint32_t f = pos + 1 > (uint32_t)p.win ? pos + 1 - p.win : 0;
-        lo[u] = sp.nc + (f - sp.wlo);
-        hi[u] = sp.nc + (pos - sp.wlo) + 1;
+        pg[i] = (blk ? btab : rtab)[r >> pl.log2page];
       }
     }
-
-    // 32 keys (tile rows from `rows`, key index j0 of the first)
-    auto keys32 = [&](const bf16_t* rows, const float* pz, bool bad, uint32_t j0) {
-      f32x4 sa[QW], sb[QW];
+  };
+  auto load_rows = [&](uint32_t t0) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        bf16x8 kf[W::NS];
-#pragma unroll
-        for (int s = 0; s < W::NS; ++s) kf[s] = *reinterpret_cast<const bf16x8*>(rows + 16 * HD * h + to.key(s));
-#pragma unroll
-        for (int u = 0; u < QW; ++u) {
-          if (h == 0) sa[u] = w[u].scores(kf);
-          else sb[u] = w[u].scores(kf);
-        }
+    for (int i = 0; i < NLD; ++i) {
+      const uint32_t j = t0 + lrow + RSTEP * i;
+      bool blk;
+      const uint32_t r = line_of(j, blk);
+      const bool ok = (unsigned)pg[i] < (unsigned)pl.P;
+      const long long pr = ok ? ((long long)pg[i] << pl.log2page) + (r & lmask) : 0;
+      pf[i] = make_uint4(0, 0, 0, 0);
+      code[i] = 127;
+      if (ok) {
+        pf[i] = *reinterpret_cast<const uint4*>(static_cast<const char*>(pl.rows) +
+                                                (pr * TPR + lch) * 16);
+        if constexpr (FMT != PF_BF16) code[i] = pl.scales[pr];
       }
-      bf16x8 pb[QW];
+    }
+  };
+  auto store_rows_lds = [&](int buf) {
+    bool bad_any = false;
+#pragma unroll
+    for (int i = 0; i < NLD; ++i) {
+      const int row = lrow + RSTEP * i;
+      bf16_t* dst = tile[buf] + row * HD;
+      const int sw = tile_swz<HD>(row & 15);
+      if constexpr (FMT == PF_BF16) {
+        const uint32_t w[4] = {pf[i].x, pf[i].y, pf[i].z, pf[i].w};
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          bad |= (w[e] & 0x7f80u) == 0x7f80u || (w[e] & 0x7f800000u) == 0x7f800000u;
+        // the whole row is bad where one of its lanes is
+        const unsigned long long g = __ballot(bad) >> (lane & ~(TPR - 1)) & ((1ull << TPR) - 1);
+        if (g) pf[i] = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(dst + 8 * (lch ^ sw)) = pf[i];
+        if (lch == 0) poison[buf][row] = g ? __uint_as_float(0x7fc00000u) : 0.f;
+        bad_any |= g != 0;
+      } else {
+        const bool bad = code[i] == kScaleNan;
+        const float sc = row_scale(bad ? 127 : code[i]);
+        const uint32_t keep = bad ? 0u : 0xffffffffu;
+        const uint2 a = dequant4_bf16<FMT>(pf[i].x & keep, sc), b = dequant4_bf16<FMT>(pf[i].y & keep, sc);
+        const uint2 c = dequant4_bf16<FMT>(pf[i].z & keep, sc), d = dequant4_bf16<FMT>(pf[i].w & keep, sc);
+        *reinterpret_cast<uint4*>(dst + 8 * ((2 * lch) ^ sw)) = make_uint4(a.x, a.y, b.x, b.y);
+        *reinterpret_cast<uint4*>(dst + 8 * ((2 * lch + 1) ^ sw)) = make_uint4(c.x, c.y, d.x, d.y);
+        if (lch == 0) poison[buf][row] = bad ? __uint_as_float(0x7fc00000u) : 0.f;
+        bad_any |= bad;
+      }
+    }
+    if (bad_any) any_bad = 1;
+  };
+
+  // the first tile's rows are in flight while the queries load
+  const uint32_t nt = (k1 - min(k0, k1) + KC - 1) / KC;
+  if (nt) {
+    load_pages(k0);
+    load_rows(k0);
+    load_pages(k0 + KC);
+  }
+
+  W w[QW];
+  uint32_t vis[QW], lo[QW], hi[QW];  // this lane's row: keys [0, vis) and [lo, hi)
+  int head[QW];
+#pragma unroll
+  for (int u = 0; u < QW; ++u) {
+    const int r = r0 + 16 * (QW * wv + u) + n;
+    const bool live = r < nrow;
+    const int rr = live ? r : nrow - 1;
+    const int tok = rr / p.nh;
+    head[u] = rr - tok * p.nh;
+    const T* qrow = static_cast<const T*>(p.q) + ((long long)sq.row0 * p.nh + rr) * HD;
+    w[u].template init_always<T>(qrow, live, p.normalize_q != 0, p.scale);
+    const uint32_t pos = sq.ctx + tok;
+    vis[u] = live ? visible_blocks(p, pos) : 0xffffffffu;  // (a padding row: never stored)
+    lo[u] = hi[u] = 0;
+    if (live && sp.nw) {
+      const uint32_t f = pos + 1 > (uint32_t)p.win ? pos + 1 - p.win : 0;
+      lo[u] = sp.nc + (f - sp.wlo);
+      hi[u] = sp.nc + (pos - sp.wlo) + 1;
+    }
+  }
+
+  // 32 keys (tile rows from `rows`, key index j0 of the first)
+  auto keys32 = [&](const bf16_t* rows, const float* pz, bool bad, uint32_t j0) {
+    f32x4 sa[QW], sb[QW];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      bf16x8 kf[W::NS];
+#pragma unroll
+      for (int s = 0; s < W::NS; ++s) kf[s] = *reinterpret_cast<const bf16x8*>(rows + 16 * HD * h + to.key(s));
 #pragma unroll
       for (int u = 0; u < QW; ++u) {
-        float sc[8] = {sa[u][0], sa[u][1], sa[u][2], sa[u][3], sb[u][0], sb[u][1], sb[u][2], sb[u][3]};
-        if (bad) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) sc[e] += pz[4 * q4 + (e < 4 ? e : 12 + e)];
-        }
-        const bool full = j0 + 32 <= k1 && (j0 + 32 <= vis[u] || (j0 >= lo[u] && j0 + 32 <= hi[u]));
-        if (__ballot(!full)) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint32_t j = j0 + 4 * q4 + (e < 4 ? e : 12 + e);
-            const bool ok = j < k1 && (j < vis[u] || (j >= lo[u] && j < hi[u]));
-            sc[e] = ok ? sc[e] : -INFINITY;
-          }
-        }
-        pb[u] = w[u].softmax32(sc);
+        if (h == 0) sa[u] = w[u].scores(kf);
+        else sb[u] = w[u].scores(kf);
       }
-#pragma unroll
-      for (int t = 0; t < W::NT; ++t) {
-        const bf16x8 va = W::vt_frag(rows, to, t);
-#pragma unroll
-        for (int u = 0; u < QW; ++u)
-          w[u].o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb[u], w[u].o[t], 0, 0, 0);
-      }
-    };
-
-    if (tid == 0) any_bad = 0;
-    __syncthreads();  // the buffers of the last row tile are free
-    if (nt) store_rows_lds(0);
-    __syncthreads();
-    for (uint32_t t = 0; t < nt; ++t) {
-      const int buf = t & 1;
-      const uint32_t j0 = k0 + t * KC;
-      if (t + 1 < nt) {
-        load_rows(j0 + KC);
-        load_pages(j0 + 2 * KC);
-      }
-      const bool bad = any_bad != 0;  // (set early for the next tile: this one's poison is 0)
-#pragma unroll
-      for (int s = 0; s < KC / 32 / KG; ++s) {
-        const int at = 32 * (s * KG + kg);
-        if (j0 + at < k1) keys32(tile[buf] + at * HD, poison[buf] + at, bad, j0 + at);
-      }
-      if (t + 1 < nt) store_rows_lds(buf ^ 1);
-      __syncthreads();
     }
-
-    // sums of the row: over its four lanes, then over the waves that shared it
-    char* const stage = reinterpret_cast<char*>(&tile[0][0]) + wv * 16 * HD * 4;
-    static_assert(NWV * 16 * HD * 4 <= (int)sizeof(tile), "the staged outputs fit in the tiles");
-#pragma unroll
-    for (int u = 0; u < QW; ++u) w[u].finalize();
-    if constexpr (KG > 1) {
-      static_assert(QW == 1, "waves that share keys take one group");
-      float* const ob = reinterpret_cast<float*>(stage);
-#pragma unroll
-      for (int t = 0; t < W::NT; ++t) *reinterpret_cast<f32x4*>(ob + (t * 64 + lane) * 4) = w[0].o[t];
-      if (q4 == 0) {
-        join_ml[wv][n][0] = w[0].M;
-        join_ml[wv][n][1] = w[0].L;
-      }
-      __syncthreads();
-      if (kg == 0) {
-        float M = w[0].M;
-#pragma unroll
-        for (int g = 1; g < KG; ++g) M = fmaxf(M, join_ml[wv + g][n][0]);
-        const float f0 = fast_exp2(w[0].M - M);
-        w[0].L *= f0;
-#pragma unroll
-        for (int t = 0; t < W::NT; ++t) w[0].o[t] *= f0;
-#pragma unroll
-        for (int g = 1; g < KG; ++g) {
-          const float f = fast_exp2(join_ml[wv + g][n][0] - M);
-          w[0].L += f * join_ml[wv + g][n][1];
-          const float* og = reinterpret_cast<const float*>(stage + g * 16 * HD * 4);
-#pragma unroll
-          for (int t = 0; t < W::NT; ++t) w[0].o[t] += f * *reinterpret_cast<const f32x4*>(og + (t * 64 + lane) * 4);
-        }
-        w[0].M = M;
-      }
-      __syncthreads();  // the partial outputs are read before their place is staged over
-      if (kg != 0) continue;
-    }
+    bf16x8 pb[QW];
 #pragma unroll
     for (int u = 0; u < QW; ++u) {
-      const int r = r0 + 16 * (QW * rg + u);
-      if (u > 0) wave_lds_sync();
-      if (r >= nrow) break;
-      const int live = min(16, nrow - r);
-      const long long g = (long long)sq.row0 * p.nh + r;
-      if (whole) {
-        const float f = w[u].finish(p.sink != nullptr, p.sink ? p.sink[head[u]] : 0.f);
-        store_rows<HD, T>(w[u].o, f, static_cast<T*>(p.out) + g * HD, live, stage);
-      } else {
-        const long long gp = (long long)blockIdx.z * pl.N * p.nh + g;
-        store_rows<HD, float>(w[u].o, 1.f, p.part_o + gp * HD, live, stage);
-        if (q4 == 0 && n < live) {
-          p.part_ml[2 * (gp + n)] = w[u].M;
-          p.part_ml[2 * (gp + n) + 1] = w[u].L;
+      float sc[8] = {sa[u][0], sa[u][1], sa[u][2], sa[u][3], sb[u][0], sb[u][1], sb[u][2], sb[u][3]};
+      if (bad) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sc[e] += pz[4 * q4 + (e < 4 ? e : 12 + e)];
+      }
+      const bool full = j0 + 32 <= k1 && (j0 + 32 <= vis[u] || (j0 >= lo[u] && j0 + 32 <= hi[u]));
+      if (__ballot(!full)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t j = j0 + 4 * q4 + (e < 4 ? e : 12 + e);
+          const bool ok = j < k1 && (j < vis[u] || (j >= lo[u] && j < hi[u]));
+          sc[e] = ok ? sc[e] : -INFINITY;
         }
       }
+      pb[u] = w[u].softmax32(sc);
     }
+#pragma unroll
+    for (int t = 0; t < W::NT; ++t) {
+      const bf16x8 va = W::vt_frag(rows, to, t);
+#pragma unroll
+      for (int u = 0; u < QW; ++u)
+        w[u].o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb[u], w[u].o[t], 0, 0, 0);
+    }
+  };
+
+  if (tid == 0) any_bad = 0;
+  __syncthreads();
+  if (nt) store_rows_lds(0);
+  __syncthreads();
+  for (uint32_t t = 0; t < nt; ++t) {
+    const int buf = t & 1;
+    const uint32_t j0 = k0 + t * KC;
+    if (t + 1 < nt) {
+      load_rows(j0 + KC);
+      load_pages(j0 + 2 * KC);
+    }
+    const bool bad = any_bad != 0;  // (set early for the next tile: this one's poison is 0)
+#pragma unroll
+    for (int s = 0; s < KC / 32; ++s) {
+      const int at = 32 * s;
+      if (j0 + at < k1) keys32(tile[buf] + at * HD, poison[buf] + at, bad, j0 + at);
+    }
+    if (t + 1 < nt) store_rows_lds(buf ^ 1);
+    __syncthreads();
+  }
+
+  char* const stage = reinterpret_cast<char*>(&tile[0][0]) + wv * 16 * HD * 4;
+  static_assert(NWV * 16 * HD * 4 <= (int)sizeof(tile), "the staged outputs fit in the tiles");
+#pragma unroll
+  for (int u = 0; u < QW; ++u) {
+    const int r = r0 + 16 * (QW * wv + u);
+    if (u > 0) wave_lds_sync();
+    if (r >= nrow) break;
+    w[u].finalize();
+    store_group<HD, T>(p, w[u], (long long)sq.row0 * p.nh + r, min(16, nrow - r), whole, head[u], stage);
   }
 }
 
 // Joins the ranges of rows that have more than one: HD / 8 lanes a row.
 template <int HD, typename T>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p, int tile_rows) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p) {
   constexpr int LPR = HD / 8;
   const PagedSeq sq = paged_seq(p.pool, blockIdx.y);
-  const int nrow = sq.len * p.nh;
+  const int nrow = computed_rows(p, sq);
   const int ch = 8 * (threadIdx.x % LPR);
   for (int r = blockIdx.x * (256 / LPR) + threadIdx.x / LPR; r < nrow; r += gridDim.x * (256 / LPR)) {
-    const int r0 = r / tile_rows * tile_rows;
-    const KeySpan sp = key_span(p, sq, r0 / p.nh, (min(r0 + tile_rows, nrow) - 1) / p.nh);
-    const uint32_t total = sp.nc + sp.nw, per = range_keys(p, total);
+    const int r0 = r / p.rows * p.rows;
+    const KeySpan sp = key_span(p, sq, r0 / p.nh, (min(r0 + p.rows, nrow) - 1) / p.nh);
+    const KeySteps ks = key_steps(p, sp);
+    const bool steps = p.rows <= kPagedTokenRows;
+    const uint32_t total = steps ? ks.nb + ks.nw : sp.nc + sp.nw, per = range_len(p, total, steps ? kStepUnit : KC);
     if (total <= per) continue;
     const int ns = (int)((total + per - 1) / per);
     const long long g = (long long)sq.row0 * p.nh + r, stride = (long long)p.pool.N * p.nh;
-    float M = kMFloor;
-    for (int s = 0; s < ns; ++s) M = fmaxf(M, p.part_ml[2 * (g + s * stride)]);
-    float L = 0.f, o[8] = {};
-    for (int s = 0; s < ns; ++s) {
-      const float* ml = p.part_ml + 2 * (g + s * stride);
-      const float f = fast_exp2(ml[0] - M);
-      float v[8];
-      Load8<float>::run(p.part_o + (g + s * stride) * HD + ch, v);
-      L = fmaf(f, ml[1], L);
+    // eight ranges' sums in flight together (past the last one it again, with weight 0)
+    float M = kMFloor, L = 0.f, o[8] = {};
+    for (int s0 = 0; s0 < ns; s0 += 8) {
+      float2 ml[8];
+      float v[8][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = fmaf(f, v[i], o[i]);
+      for (int s = 0; s < 8; ++s) {
+        const long long at = g + min(s0 + s, ns - 1) * stride;
+        ml[s] = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
+        Load8<float>::run(p.part_o + at * HD + ch, v[s]);
+      }
+      float mx = M;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) mx = fmaxf(mx, ml[s].x);
+      const float f0 = fast_exp2(M - mx);
+      L *= f0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] *= f0;
+      M = mx;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        if (s0 + s >= ns) break;
+        const float f = fast_exp2(ml[s].x - M);
+        L = fmaf(f, ml[s].y, L);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = fmaf(f, v[s][i], o[i]);
+      }
     }
     float den = L;
     if (p.sink) den += fast_exp2(p.sink[r % p.nh] * kLog2eF - M);
@@ -370,34 +688,34 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p, int 
   }
 }
 
-// Row groups of a workgroup for rows query rows a sequence: all of them up to 4
-// groups (fewer groups leave waves to split the keys), else 8.
-int row_groups(long long rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8; }
-
 template <int HD, int FMT, typename T>
-void attn_launch(const PagedAttnParams& p, int rows, hipStream_t s) {
+void attn_launch(const PagedAttnParams& p, hipStream_t s) {
   const long long nrow = (long long)p.max_len * p.nh;
-  const dim3 grid((unsigned)((nrow + rows - 1) / rows), (unsigned)(p.pool.S + (p.zero_tail ? 1 : 0)),
+  const dim3 grid((unsigned)((nrow + p.rows - 1) / p.rows), (unsigned)(p.pool.S + (p.zero_tail ? 1 : 0)),
                   (unsigned)p.nsplit);
-#define KCH_PA(RG, QW, KG) \
-  hipLaunchKernelGGL((paged_attn_kernel<HD, FMT, RG, QW, KG, T>), grid, dim3(64 * RG / QW * KG), 0, s, p)
-  if (rows == 16) KCH_PA(1, 1, 4);
-  else if (rows == 32) KCH_PA(2, 1, 2);
-  else if (rows == 64) KCH_PA(4, 1, 1);
-  else KCH_PA(8, 1, 1);
+  const bool big = p.pool.log2page >= 5;
+#define KCH_PT(QW, BIG) hipLaunchKernelGGL((paged_token_kernel<HD, FMT, QW, BIG, T>), grid, dim3(256), 0, s, p)
+#define KCH_PA(RG, QW) hipLaunchKernelGGL((paged_attn_kernel<HD, FMT, RG, QW, T>), grid, dim3(64 * RG / QW), 0, s, p)
+  if (p.rows == 16 && big) KCH_PT(1, true);
+  else if (p.rows == 16) KCH_PT(1, false);
+  else if (p.rows == 32 && big) KCH_PT(2, true);
+  else if (p.rows == 32) KCH_PT(2, false);
+  else if (p.rows == 64) KCH_PA(4, 1);
+  else KCH_PA(8, 1);
+#undef KCH_PT
 #undef KCH_PA
   if (p.nsplit > 1) {
     constexpr int RPB = 256 / (HD / 8);
     const dim3 jg((unsigned)((nrow + RPB - 1) / RPB), (unsigned)p.pool.S);
-    hipLaunchKernelGGL((paged_join_kernel<HD, T>), jg, dim3(256), 0, s, p, rows);
+    hipLaunchKernelGGL((paged_join_kernel<HD, T>), jg, dim3(256), 0, s, p);
   }
 }
 
 template <int HD, int FMT>
-void attn_launch_t(const PagedAttnParams& p, int dtype, int rows, hipStream_t s) {
-  if (dtype == DT_BF16) attn_launch<HD, FMT, bf16_t>(p, rows, s);
-  else if (dtype == DT_F16) attn_launch<HD, FMT, _Float16>(p, rows, s);
-  else attn_launch<HD, FMT, float>(p, rows, s);
+void attn_launch_t(const PagedAttnParams& p, int dtype, hipStream_t s) {
+  if (dtype == DT_BF16) attn_launch<HD, FMT, bf16_t>(p, s);
+  else if (dtype == DT_F16) attn_launch<HD, FMT, _Float16>(p, s);
+  else attn_launch<HD, FMT, float>(p, s);
 }
 
 }  // namespace
@@ -405,30 +723,32 @@ void attn_launch_t(const PagedAttnParams& p, int dtype, int rows, hipStream_t s)
 PagedAttnPlan paged_attn_plan(int S, int N, int nh, int c, int m2, int win, int max_len, int max_ctx) {
   PagedAttnPlan pl;
   const long long nrow = (long long)max_len * nh;
-  pl.rows = 16 * row_groups(nrow);
+  pl.rows = nrow <= 16 ? 16 : nrow <= 32 ? 32 : nrow <= 64 ? 64 : 128;
+  const bool steps = pl.rows <= kPagedTokenRows;
   const long long tiles = (nrow + pl.rows - 1) / pl.rows * S;
   const long long keys = ((long long)max_ctx + max_len) / m2 + win + (pl.rows + nh - 1) / nh;
-  // two workgroups for each of 256 CUs; a range no shorter than four tiles
-  const long long want = 512 / (tiles > 0 ? tiles : 1);
-  long long per = want > 1 ? (keys + want - 1) / want : keys;
-  per = ((per < 4 * KC ? 4 * KC : per) + KC - 1) / KC * KC;
-  pl.nsplit = (int)((keys + per - 1) / per);
+  // units of a range: 32-key steps, or keys, a tile at a time
+  const long long unit = steps ? kStepUnit : KC, total = steps ? keys / 32 + 3 : keys;
+  // workgroups for each of 256 CUs, and no range too short to be worth its join
+  const long long want = (pl.rows == 16 ? 768 : 512) / (tiles > 0 ? tiles : 1), least = steps ? 2 * kStepUnit : 4 * KC;
+  long long per = want > 1 ? (total + want - 1) / want : total;
+  per = ((per < least ? least : per) + unit - 1) / unit * unit;
+  pl.nsplit = (int)((total + per - 1) / per);
   if (pl.nsplit < 1) pl.nsplit = 1;
-  pl.split_keys = (int)(per < (1ll << 30) ? per : (1ll << 30));
+  pl.range = (int)(per < (1ll << 30) ? per : (1ll << 30));
   pl.bytes = pl.nsplit > 1 ? (size_t)pl.nsplit * N * nh * (c + 2) * sizeof(float) : 0;
   return pl;
 }
 
-hipError_t paged_attn_dispatch(const PagedAttnParams& p, const PagedAttnPlan& plan, int format, int dtype,
-                               hipStream_t s) {
+hipError_t paged_attn_dispatch(const PagedAttnParams& p, int format, int dtype, hipStream_t s) {
   if (p.pool.c == 128) {
-    if (format == PF_BF16) attn_launch_t<128, PF_BF16>(p, dtype, plan.rows, s);
-    else if (format == PF_E4M3) attn_launch_t<128, PF_E4M3>(p, dtype, plan.rows, s);
-    else attn_launch_t<128, PF_INT8>(p, dtype, plan.rows, s);
+    if (format == PF_BF16) attn_launch_t<128, PF_BF16>(p, dtype, s);
+    else if (format == PF_E4M3) attn_launch_t<128, PF_E4M3>(p, dtype, s);
+    else attn_launch_t<128, PF_INT8>(p, dtype, s);
   } else {
-    if (format == PF_BF16) attn_launch_t<64, PF_BF16>(p, dtype, plan.rows, s);
-    else if (format == PF_E4M3) attn_launch_t<64, PF_E4M3>(p, dtype, plan.rows, s);
-    else attn_launch_t<64, PF_INT8>(p, dtype, plan.rows, s);
+    if (format == PF_BF16) attn_launch_t<64, PF_BF16>(p, dtype, s);
+    else if (format == PF_E4M3) attn_launch_t<64, PF_E4M3>(p, dtype, s);
+    else attn_launch_t<64, PF_INT8>(p, dtype, s);
   }
   return hipGetLastError();
 }
