@@ -214,23 +214,20 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
         }
       }
     };
-    // two steps in flight, and the table entries of the two after them. The loads keep
-    // this order everywhere: a wait counts the loads issued after the one it waits for.
-    int pa[NP], pb[NP];
-    Step sa, sb;
+    // a step in flight, and the table entry of the one after it. The loads keep this
+    // order everywhere: a wait counts the loads issued after the one it waits for.
+    int pg[NP];
+    Step sa;
     int st = s0 + wv;
-    auto next = [&](int at, int (&pg)[NP], Step& s) {
+    auto next = [&](int at) {
       __builtin_amdgcn_sched_barrier(0);
-      load_step(at, pg, s);
+      load_step(at, pg, sa);
       __builtin_amdgcn_sched_barrier(0);
-      load_page(at + 8, pg);
+      load_page(at + 4, pg);
       __builtin_amdgcn_sched_barrier(0);
     };
-    load_page(st, pa);
-    __builtin_amdgcn_sched_barrier(0);
-    load_page(st + 4, pb);
-    next(st, pa, sa);
-    next(st + 4, pb, sb);
+    load_page(st, pg);
+    next(st);
 
     // the queries, while the first steps' rows are in flight; this lane's row sees
     // block rows below vis, and window rows [lo, hi) counted from the first window step's
@@ -259,7 +256,7 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
       const bool blk = d < 0;
       const uint32_t j0 = 32 * (blk ? st : d);  // block row, or window row, of the step's first
       // rows that no query of the workgroup sees, or that are none of the pool: zeros
-      const uint32_t ua = blk ? 0 : ks.woff, ub = st > last ? 0 : blk ? sp.nc : ks.woff + sp.nw;
+      const uint32_t ua = blk ? 0 : ks.woff, ub = blk ? sp.nc : ks.woff + sp.nw;
       if (!(BIG && s.ok && j0 >= ua && j0 + 32 <= ub)) {
 #pragma unroll
         for (int i = 0; i < NLI; ++i) {
@@ -334,7 +331,7 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
 #pragma unroll
           for (int e = 0; e < 8; ++e) sc[e] += poison[wv][4 * q4 + (e < 4 ? e : 12 + e)];
         }
-        const uint32_t la = blk ? 0 : lo[u], lb = st > last ? 0 : blk ? vis[u] : hi[u];
+        const uint32_t la = blk ? 0 : lo[u], lb = blk ? vis[u] : hi[u];
         if (__ballot(j0 < la || j0 + 32 > lb)) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
@@ -353,17 +350,12 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
       }
     };
 
-    // A step's registers are free once it is in LDS: the load of the one after the next
-    // goes out before the products. Steps go in pairs, the second one past the range
-    // as one without keys (an exit between them would have the loop's first wait drain
-    // every load).
-    for (; st <= last; st += 8) {
+    // a step's registers are free once it is in LDS: the next one's load goes out before
+    // the products
+    for (; st <= last; st += 4) {
       put(st, sa);
-      next(st + 8, pa, sa);
+      next(st + 4);
       use(st);
-      put(st + 4, sb);
-      next(st + 12, pb, sb);
-      use(st + 4);
     }
   } else {
 #pragma unroll
