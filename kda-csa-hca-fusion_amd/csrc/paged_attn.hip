@@ -403,6 +403,21 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
   }
 }
 
+// The keys below k1 that a token of a tile sees: [0, vis) and [lo, hi). All grow with the
+// token.
+struct RowKeys {
+  uint32_t vis, lo, hi;
+};
+__device__ __forceinline__ RowKeys row_keys(const PagedAttnParams& p, const PagedSeq& sq, const KeySpan& sp,
+                                            int tok, uint32_t k1) {
+  const uint32_t pos = sq.ctx + tok, f = pos + 1 > (uint32_t)p.win ? pos + 1 - p.win : 0;
+  RowKeys k;
+  k.vis = min(visible_blocks(p, pos), k1);
+  k.lo = sp.nw ? min(sp.nc + (f - sp.wlo), k1) : 0;
+  k.hi = sp.nw ? min(sp.nc + (pos - sp.wlo) + 1, k1) : 0;
+  return k;
+}
+
 // RG groups of 16 rows of a sequence, QW of them a wave, and a range of keys. Two
 // workgroups of 8 waves a CU (128 registers): 132 us where one took 156, for 8 chunks of up
 // to 2048 tokens behind 128K.
@@ -533,6 +548,8 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
 
   W w[QW];
   uint32_t vis[QW], lo[QW], hi[QW];  // this lane's row: keys [0, vis) and [lo, hi)
+  RowKeys first[QW], final_[QW];
+  bool seen[QW];
   int head[QW];
 #pragma unroll
   for (int u = 0; u < QW; ++u) {
@@ -543,14 +560,16 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
     head[u] = rr - tok * p.nh;
     const T* qrow = static_cast<const T*>(p.q) + ((long long)sq.row0 * p.nh + rr) * HD;
     w[u].template init_always<T>(qrow, live, p.normalize_q != 0, p.scale);
-    const uint32_t pos = sq.ctx + tok;
-    vis[u] = live ? visible_blocks(p, pos) : 0xffffffffu;  // (a padding row: never stored)
-    lo[u] = hi[u] = 0;
-    if (live && sp.nw) {
-      const uint32_t f = pos + 1 > (uint32_t)p.win ? pos + 1 - p.win : 0;
-      lo[u] = sp.nc + (f - sp.wlo);
-      hi[u] = sp.nc + (pos - sp.wlo) + 1;
-    }
+    const RowKeys k = row_keys(p, sq, sp, tok, k1);
+    // (a padding row is never stored: it masks nothing)
+    vis[u] = live ? k.vis : k1;
+    lo[u] = k.lo;
+    hi[u] = k.hi;
+    // the group's first and last rows bound what its rows see
+    const int g0 = r0 + 16 * (QW * wv + u), g1 = min(g0 + 15, nrow - 1);
+    seen[u] = g0 < nrow;
+    first[u] = row_keys(p, sq, sp, min(g0, nrow - 1) / p.nh, k1);
+    final_[u] = row_keys(p, sq, sp, g1 / p.nh, k1);
   }
 
   // 32 keys (tile rows from `rows`, key index j0 of the first)
@@ -575,12 +594,11 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
 #pragma unroll
         for (int e = 0; e < 8; ++e) sc[e] += pz[4 * q4 + (e < 4 ? e : 12 + e)];
       }
-      const bool full = j0 + 32 <= k1 && (j0 + 32 <= vis[u] || (j0 >= lo[u] && j0 + 32 <= hi[u]));
-      if (__ballot(!full)) {
+      if (!(j0 + 32 <= first[u].vis || (j0 >= final_[u].lo && j0 + 32 <= first[u].hi))) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const uint32_t j = j0 + 4 * q4 + (e < 4 ? e : 12 + e);
-          const bool ok = j < k1 && (j < vis[u] || (j >= lo[u] && j < hi[u]));
+          const bool ok = (j < vis[u]) | (j - lo[u] < hi[u] - lo[u]);
           sc[e] = ok ? sc[e] : -INFINITY;
         }
       }
@@ -610,7 +628,12 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
 #pragma unroll
     for (int s = 0; s < KC / 32; ++s) {
       const int at = 32 * s;
-      if (j0 + at < k1) keys32(tile[buf] + at * HD, poison[buf] + at, bad, j0 + at);
+      // (a step that none of the wave's rows sees is passed over)
+      bool some = false;
+#pragma unroll
+      for (int u = 0; u < QW; ++u)
+        some |= seen[u] && (j0 + at < final_[u].vis || (j0 + at < final_[u].hi && j0 + at + 32 > first[u].lo));
+      if (some) keys32(tile[buf] + at * HD, poison[buf] + at, bad, j0 + at);
     }
     if (t + 1 < nt) store_rows_lds(buf ^ 1);
     __syncthreads();
