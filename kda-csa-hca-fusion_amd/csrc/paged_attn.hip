@@ -604,6 +604,9 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
       }
       pb[u] = w[u].softmax32(sc);
     }
+    // a wave at its products goes before those at their softmax (8 short-context chunks
+    // 82.6 -> 76.8 us, long ones 126 -> 122)
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int t = 0; t < W::NT; ++t) {
       const bf16x8 va = W::vt_frag(rows, to, t);
@@ -611,6 +614,7 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
       for (int u = 0; u < QW; ++u)
         w[u].o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb[u], w[u].o[t], 0, 0, 0);
     }
+    __builtin_amdgcn_s_setprio(0);
   };
 
   if (tid == 0) any_bad = 0;
