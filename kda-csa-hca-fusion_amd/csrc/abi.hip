@@ -1632,8 +1632,11 @@ int kch_hca_paged_attn(const void* q, const float* sink, void* out, const void* 
                 nrp * page);
   if (win > 0 && nrp == 0) return fail(KCH_ERR_INVALID, "%s: win=%d without a ring", fn, win);
   if (N == 0 || ((S == 0 || max_len == 0) && !zero_tail)) return KCH_OK;
-  if (!q || !out || !slots || !cu || !ctx) return fail(KCH_ERR_INVALID, "%s: null pointer", fn);
+  if (!q || !out || (S > 0 && (!slots || !cu || !ctx))) return fail(KCH_ERR_INVALID, "%s: null pointer", fn);
   if (((uintptr_t)q | (uintptr_t)out) & 15) return fail(KCH_ERR_INVALID, "%s: q and out must be 16-byte aligned", fn);
+  if (S == 0)  // no sequence: every row is behind the last one
+    return hip_status(fn, kch::fill_u32(out, (long long)N * nh * c / (dtype == KCH_DT_F32 ? 1 : 2), 0u,
+                                        (hipStream_t)stream));
   if (max_len > N) max_len = N;
   if (max_len < 1) max_len = 1;
   const kch::PagedAttnPlan pl = kch::paged_attn_plan(S, N, nh, c, m2, win, max_len, max_ctx);
@@ -1659,8 +1662,11 @@ int kch_paged_read(const void* rows, const void* scales, const int* table, const
   if (rc) return rc;
   if (!dtype_ok(odtype)) return fail(KCH_ERR_INVALID, "%s: unknown dtype %d", fn, odtype);
   if (N == 0 || (S == 0 && !zero_tail)) return KCH_OK;
-  if (!out || !cu) return fail(KCH_ERR_INVALID, "%s: null pointer", fn);
+  if (!out || (S > 0 && !cu)) return fail(KCH_ERR_INVALID, "%s: null pointer", fn);
   if ((uintptr_t)out & 15) return fail(KCH_ERR_INVALID, "%s: out must be 16-byte aligned", fn);
+  if (S == 0)  // no sequence: every row is behind the last one, and no row of the pool is read
+    return hip_status(fn, kch::fill_u32(out, (long long)N * c / (odtype == KCH_DT_F32 ? 1 : 2), 0u,
+                                        (hipStream_t)stream));
   p.out = out;
   p.zero_tail = zero_tail;
   return hip_status(fn, kch::paged_read_dispatch(p, format, odtype, (hipStream_t)stream));

@@ -281,71 +281,113 @@ void append_launch(const PagedAppendParams& p, int dtype, hipStream_t s) {
 }
 
 // paged_read_kernel: output row j of a sequence is row (first + j) % capacity of
-// its slot's table. 16 channels a lane; a workgroup takes kReadRows consecutive
-// output rows, whose sequences it finds by counting the entries of cu up to them
-// (64 a wave instruction) and then walks.
+// its slot's table. A workgroup takes kReadRows consecutive output rows: a thread
+// a row finds its sequence (counting the entries of cu up to the first row, 64 a wave
+// instruction, then walking) and its pool row, into LDS; then the rows stream
+// through, 16 channels a lane, all of a thread's loads before its first store. Bound by
+// the bytes: 16 caches of up to 1M tokens as bf16, 49 MB, in 12 us, 4.1 TB/s (with a lane
+// looking its rows up one after the other 13.3).
 constexpr int kReadRows = 128;
+
+template <typename OT> __device__ __forceinline__ void store16(OT* p, const float* f) {
+  if constexpr (sizeof(OT) == 4) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+  } else {
+    typedef OT v8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+    for (int i = 0; i < 16; i += 8) {
+      v8 v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (OT)f[i + e];
+      *reinterpret_cast<v8*>(p + i) = v;
+    }
+  }
+}
 
 template <int HD, int FMT, typename OT>
 __global__ __launch_bounds__(256) void paged_read_kernel(PagedReadParams p) {
-  constexpr int LPR = HD / 16, RSTEP = 256 / LPR;
+  constexpr int LPR = HD / 16, RSTEP = 256 / LPR, NR = kReadRows / RSTEP;
+  constexpr int NV = FMT == PF_BF16 ? 2 : 1;  // 16-byte loads of a lane's 16 channels
+  constexpr long long kZero = -1, kSkip = -2;
   typedef typename PagedFmt<FMT>::elem elem;
+  __shared__ long long src_row[kReadRows];
   const PagedPool& pl = p.pool;
-  const int lane = lane_id(), ch = 16 * (threadIdx.x % LPR);
-  const int base = blockIdx.x * kReadRows;
-  int seq = -1;  // the last sequence that starts at or before row `base`
-  for (int i = 0; i <= pl.S; i += 64) {
-    const bool le = i + lane <= pl.S && pl.cu[i + lane] <= base;
-    const int n = __popcll(__ballot(le));
-    seq += n;
-    if (n < 64) break;
-  }
-  const uint32_t cap = (uint32_t)pl.nbp << pl.log2page;
-  OT* out = static_cast<OT*>(p.out);
-#pragma unroll 4
-  for (int k = 0; k < kReadRows / RSTEP; ++k) {
-    const int row = base + k * RSTEP + (int)threadIdx.x / LPR;
-    if (row >= pl.N) break;
-    while (seq + 1 <= pl.S && pl.cu[seq + 1] <= row) ++seq;
-    long long pr = -1;
-    if (seq >= 0 && seq < pl.S) {
-      const int slot = pl.slots[seq];
-      const uint32_t first = pl.ctx ? pl.ctx[seq] : 0, at = row - pl.cu[seq];
-      if (cap > 0 && (unsigned)slot < (unsigned)pl.n_slots)
-        pr = pool_row(pl, pl.block_table, pl.nbp, slot, (first + at) % cap);
-    } else if (!p.zero_tail) {
-      continue;
+  const int lane = lane_id(), base = blockIdx.x * kReadRows;
+  if (threadIdx.x < kReadRows) {
+    const int row = base + threadIdx.x;
+    long long pr = kSkip;
+    int seq = -1;  // the last sequence that starts at or before row `base`
+    for (int i = 0; i <= pl.S; i += 64) {
+      const bool le = i + lane <= pl.S && pl.cu[i + lane] <= base;
+      const int n = __popcll(__ballot(le));
+      seq += n;
+      if (n < 64) break;
     }
-    float f[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = 0.f;
-    if (pr >= 0) {
-      const elem* src = static_cast<const elem*>(pl.rows) + pr * HD + ch;
-      if constexpr (FMT == PF_BF16) {
-        Load8<bf16_t>::run(src, f);
-        Load8<bf16_t>::run(src + 8, f + 8);
-      } else {
-        const uint4 w = *reinterpret_cast<const uint4*>(src);
-        const float sc = row_scale(pl.scales[pr]);
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (FMT == PF_E4M3) {
-            const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(ww[i], false);
-            const auto b = __builtin_amdgcn_cvt_pk_f32_fp8(ww[i], true);
-            f[4 * i] = a[0]; f[4 * i + 1] = a[1]; f[4 * i + 2] = b[0]; f[4 * i + 3] = b[1];
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f[4 * i + e] = (float)(int8_t)(ww[i] >> (8 * e));
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] *= sc;
+    if (row < pl.N) {
+      while (seq + 1 <= pl.S && pl.cu[seq + 1] <= row) ++seq;
+      if (seq >= 0 && seq < pl.S) {
+        const uint32_t cap = (uint32_t)pl.nbp << pl.log2page;
+        const int slot = pl.slots[seq];
+        const uint32_t first = pl.ctx ? pl.ctx[seq] : 0, at = row - pl.cu[seq];
+        pr = kZero;
+        if (cap > 0 && (unsigned)slot < (unsigned)pl.n_slots)
+          pr = pool_row(pl, pl.block_table, pl.nbp, slot, (first + at) % cap);
+      } else if (p.zero_tail) {
+        pr = kZero;
       }
     }
-    OT* dst = out + (size_t)row * HD + ch;
+    src_row[threadIdx.x] = pr;
+  }
+  __syncthreads();
+  const int lr = threadIdx.x / LPR, ch = 16 * (threadIdx.x % LPR);
+  uint4 v[NR][NV];
+  int code[NR];
+  long long pr[NR];
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) Store4<OT>::run(dst + i, f32x4{f[i], f[i + 1], f[i + 2], f[i + 3]}, 1.f);
+  for (int k = 0; k < NR; ++k) {
+    pr[k] = src_row[k * RSTEP + lr];
+    const long long at = pr[k] < 0 ? 0 : pr[k];  // (row 0 of the pool is there: P >= 1)
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const elem*>(pl.rows) + at * HD + ch);
+#pragma unroll
+    for (int e = 0; e < NV; ++e) v[k][e] = src[e];
+    if constexpr (FMT != PF_BF16) code[k] = pl.scales[at];
+  }
+#pragma unroll
+  for (int k = 0; k < NR; ++k) {
+    if (pr[k] == kSkip) continue;
+    float f[16];
+    if constexpr (FMT == PF_BF16) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t w[4] = {v[k][e].x, v[k][e].y, v[k][e].z, v[k][e].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f[8 * e + 2 * i] = __uint_as_float(w[i] << 16);
+          f[8 * e + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+      }
+    } else {
+      const uint32_t w[4] = {v[k][0].x, v[k][0].y, v[k][0].z, v[k][0].w};
+      const float sc = row_scale(code[k]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (FMT == PF_E4M3) {
+          const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], false);
+          const auto b = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], true);
+          f[4 * i] = a[0]; f[4 * i + 1] = a[1]; f[4 * i + 2] = b[0]; f[4 * i + 3] = b[1];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f[4 * i + e] = (float)(int8_t)(w[i] >> (8 * e));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f[i] *= sc;
+    }
+    if (pr[k] == kZero)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f[i] = 0.f;
+    store16<OT>(static_cast<OT*>(p.out) + (size_t)(base + k * RSTEP + lr) * HD + ch, f);
   }
 }
 

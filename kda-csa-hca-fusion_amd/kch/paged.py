@@ -38,58 +38,74 @@ def _fail(fn, msg):
     raise ValueError(f"{fn}: {msg}")
 
 
-# The checks of a step's tensors are single expressions over attributes of about 50 ns
-# each, with the message made only where one fails: a decode step pays them per layer.
-
-def _is_ints(t, dim, dev):
-    return t.dtype is _I32 and t.dim() == dim and t.is_contiguous() and t.get_device() == dev
-
-
 def _need_ints(fn, name, t, dim, dev):
-    if not _is_ints(t, dim, dev):
+    if t.dtype is not _I32 or t.dim() != dim or not t.is_contiguous() or t.get_device() != dev:
         _fail(fn, f"{name} must be a contiguous int32 tensor of {dim} dimension(s) on cuda:{dev}, got "
                   f"{t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _pool(fn, rows, scales):
-    """(format, P, page, c, device index) of a pool after its checks."""
-    fmt = _FORMATS.get(rows.dtype)
-    if fmt is None:
+def _explain(fn, rows, scales, block_table, ring_table, slots, cu_seqlens, ctx_lens):
+    """Raises for the first thing wrong with a step's tensors."""
+    _lib.require_gpu(fn, rows)
+    if rows.dtype not in _FORMATS:
         raise TypeError(f"{fn}: rows must be bfloat16, float8_e4m3fn or int8, got {rows.dtype}")
     if rows.dim() != 3 or not rows.is_contiguous():
         _fail(fn, f"rows must be a contiguous [pages, page, c] tensor, got {tuple(rows.shape)}")
-    P, page, c = rows.shape
     dev = rows.get_device()
-    if fmt and (scales is None or scales.dtype is not torch.uint8 or scales.shape != (P, page)
-                or not scales.is_contiguous() or scales.get_device() != dev):
-        _fail(fn, f"8-bit rows need scales, contiguous uint8 [{P}, {page}] on {rows.device}")
-    return fmt, P, page, c, dev
-
-
-def _step(fn, dev, slots, cu_seqlens, ctx_lens):
-    S = slots.shape[0]
-    if not (_is_ints(slots, 1, dev) and _is_ints(cu_seqlens, 1, dev) and cu_seqlens.shape[0] == S + 1
-            and (ctx_lens is None or (_is_ints(ctx_lens, 1, dev) and ctx_lens.shape[0] == S))):
-        for name, t in (("slots", slots), ("cu_seqlens", cu_seqlens), ("ctx_lens", ctx_lens)):
-            if t is not None:
-                _need_ints(fn, name, t, 1, dev)
-        if cu_seqlens.shape[0] != S + 1:
-            _fail(fn, f"cu_seqlens has {cu_seqlens.shape[0]} entries for {S} sequences")
-        _fail(fn, f"ctx_lens has {ctx_lens.shape[0]} entries for {S} sequences")
-    return S
-
-
-def _tables(fn, dev, block_table, ring_table):
-    """(slots, block pages, ring pages) of the tables."""
+    if rows.dtype is not torch.bfloat16 and (
+            scales is None or scales.dtype is not torch.uint8 or scales.shape != rows.shape[:2]
+            or not scales.is_contiguous() or scales.get_device() != dev):
+        _fail(fn, f"8-bit rows need scales, contiguous uint8 {tuple(rows.shape[:2])} on {rows.device}")
     _need_ints(fn, "block_table", block_table, 2, dev)
-    n_slots, nbp = block_table.shape
-    if ring_table is None:
-        return n_slots, nbp, 0
-    _need_ints(fn, "ring_table", ring_table, 2, dev)
-    m, nrp = ring_table.shape
-    if m != n_slots:
-        _fail(fn, f"ring_table has {m} slots, block_table {n_slots}")
-    return n_slots, nbp, nrp
+    if ring_table is not None:
+        _need_ints(fn, "ring_table", ring_table, 2, dev)
+        if ring_table.shape[0] != block_table.shape[0]:
+            _fail(fn, f"ring_table has {ring_table.shape[0]} slots, block_table {block_table.shape[0]}")
+    S = slots.shape[0] if slots.dim() else 0
+    for name, t, n in (("slots", slots, S), ("cu_seqlens", cu_seqlens, S + 1), ("ctx_lens", ctx_lens, S)):
+        if t is not None:
+            _need_ints(fn, name, t, 1, dev)
+            if t.shape[0] != n:
+                _fail(fn, f"{name} has {t.shape[0]} entries for {S} sequences")
+    raise AssertionError(fn)
+
+
+def _step(fn, rows, scales, block_table, ring_table, slots, cu_seqlens, ctx_lens):
+    """(format, device index, P, page, c, slots, block pages, ring pages, S) of a step after its
+    checks. One expression over attributes of some 50 ns each, which a decode step pays
+    per layer and call; what is wrong is looked for only where it fails."""
+    i32 = _I32
+    dev = rows.get_device()
+    fmt = _FORMATS.get(rows.dtype, -1)
+    S = -1
+    if (fmt >= 0 and dev >= 0 and rows.dim() == 3 and rows.is_contiguous()
+            and block_table.dtype is i32 and block_table.dim() == 2 and block_table.get_device() == dev
+            and block_table.is_contiguous()
+            and slots.dtype is i32 and slots.dim() == 1 and slots.get_device() == dev and slots.is_contiguous()
+            and cu_seqlens.dtype is i32 and cu_seqlens.dim() == 1 and cu_seqlens.get_device() == dev
+            and cu_seqlens.is_contiguous()):
+        P, page, c = rows.shape
+        n_slots, nbp = block_table.shape
+        nrp = 0
+        S, = slots.shape
+        if (cu_seqlens.shape[0] != S + 1
+                or (ctx_lens is not None and not (
+                    ctx_lens.dtype is i32 and ctx_lens.dim() == 1 and ctx_lens.get_device() == dev
+                    and ctx_lens.is_contiguous() and ctx_lens.shape[0] == S))
+                or (fmt and (scales is None or scales.dtype is not torch.uint8 or scales.get_device() != dev
+                             or not scales.is_contiguous() or scales.shape != (P, page)))):
+            S = -1
+        elif ring_table is not None:
+            if (ring_table.dtype is i32 and ring_table.dim() == 2 and ring_table.get_device() == dev
+                    and ring_table.is_contiguous()):
+                m, nrp = ring_table.shape
+                if m != n_slots:
+                    S = -1
+            else:
+                S = -1
+    if S < 0:
+        _explain(fn, rows, scales, block_table, ring_table, slots, cu_seqlens, ctx_lens)
+    return fmt, dev, P, page, c, n_slots, nbp, nrp, S
 
 
 def _rows2d(x):
@@ -124,22 +140,20 @@ def hca_paged_append(C, Z, B_pos, rows, scales, state, block_table, ring_table, 
     may occur once.
     """
     fn = "hca_paged_append"
-    if not (C.is_cuda and Z.is_cuda and rows.is_cuda):
-        _lib.require_gpu(fn, C, Z, rows)
-    fmt, P, page, c, dev = _pool(fn, rows, scales)
+    fmt, dev, P, page, c, n_slots, nbp, nrp, S = _step(fn, rows, scales, block_table, ring_table, slots,
+                                                       cu_seqlens, ctx_lens)
     if C.dim() != 2 or C.shape != Z.shape or C.shape[1] != c or C.dtype is not Z.dtype \
             or C.get_device() != dev or Z.get_device() != dev:
+        _lib.require_gpu(fn, C, Z)
         _fail(fn, f"C and Z must be [N, {c}] of one dtype on {rows.device}, got {tuple(C.shape)} {C.dtype} and "
                   f"{tuple(Z.shape)} {Z.dtype}")
     if m2 < 1:
         _fail(fn, f"m2={m2} must be >= 1")
     if B_pos.shape != (m2, c):
         _fail(fn, f"B_pos.shape={tuple(B_pos.shape)} must equal (m2, c)=({m2}, {c})")
-    n_slots, nbp, nrp = _tables(fn, dev, block_table, ring_table)
     if state.dtype is not torch.float32 or state.shape != (n_slots, 3, c) or not state.is_contiguous() \
             or state.get_device() != dev:
         _fail(fn, f"state must be contiguous float32 [{n_slots}, 3, {c}] on {rows.device}")
-    S = _step(fn, dev, slots, cu_seqlens, ctx_lens)
     if max_len < 0 or (nrp and max_len > nrp * page):
         _fail(fn, f"max_len={max_len} must be at most the ring's {nrp * page} rows")
     code = _lib.dtype_code(fn, C.dtype)
@@ -166,19 +180,17 @@ def hca_paged_attention(q, rows, scales, block_table, ring_table, slots, cu_seql
     The products are bf16 with fp32 sums whatever ``q``'s type.
     """
     fn = "hca_paged_attention"
-    if not (q.is_cuda and rows.is_cuda):
-        _lib.require_gpu(fn, q, rows)
-    fmt, P, page, c, dev = _pool(fn, rows, scales)
-    if q.dim() != 3 or q.shape[2] != c or q.shape[1] < 1 or q.get_device() != dev:
+    fmt, dev, P, page, c, n_slots, nbp, nrp, S = _step(fn, rows, scales, block_table, ring_table, slots,
+                                                       cu_seqlens, ctx_lens)
+    N, nh, width = q.shape if q.dim() == 3 else (0, 0, 0)
+    if width != c or nh < 1 or q.get_device() != dev:
+        _lib.require_gpu(fn, q)
         _fail(fn, f"q must be [N, nh, {c}] on {rows.device}, got {tuple(q.shape)} on {q.device}")
-    N, nh, _ = q.shape
     code = _lib.dtype_code(fn, q.dtype)
     if m2 < 1:
         _fail(fn, f"m2={m2} must be >= 1")
     if sliding_window < 0:
         _fail(fn, f"sliding_window={sliding_window} must be >= 0 (0 disables the branch)")
-    n_slots, nbp, nrp = _tables(fn, dev, block_table, ring_table)
-    S = _step(fn, dev, slots, cu_seqlens, ctx_lens)
     if max_len < 0 or (sliding_window and sliding_window + max_len - 1 > nrp * page):
         _fail(fn, f"sliding_window={sliding_window} and max_len={max_len} need a ring of "
                   f"{sliding_window + max_len - 1} rows, it has {nrp * page}")
@@ -197,11 +209,11 @@ def hca_paged_attention(q, rows, scales, block_table, ring_table, slots, cu_seql
     tail = 0
     if out is None:
         tail = 1
-        out = torch.empty(N, nh, c, device=rows.device, dtype=q.dtype)
+        out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != dev \
             or not out.is_contiguous() or out.data_ptr() % 16:
         _fail(fn, f"out must be a contiguous, 16-byte aligned {tuple(q.shape)} {q.dtype} tensor on {rows.device}")
-    nbytes = _lib.load().kch_hca_paged_attn_ws_bytes(S, N, nh, c, m2, sliding_window, max_len, max_ctx)
+    nbytes = (_lib._lib or _lib.load()).kch_hca_paged_attn_ws_bytes(S, N, nh, c, m2, sliding_window, max_len, max_ctx)
     ws = torch.empty(nbytes, device=rows.device, dtype=torch.uint8) if nbytes else None
     _lib.call_on(dev, "kch_hca_paged_attn", q.data_ptr(), _p(sink_logits), out.data_ptr(), rows.data_ptr(),
                  _p(scales), block_table.data_ptr(), _p(ring_table), slots.data_ptr(), cu_seqlens.data_ptr(),
@@ -216,11 +228,7 @@ def paged_read(rows, scales, table, slots, cu_rows, *, total, first=None, dtype=
     table), capacity its pages times their rows. ``total`` is the number of result rows; those
     behind the last sequence are zeros (in ``out`` as they were)."""
     fn = "paged_read"
-    if not rows.is_cuda:
-        _lib.require_gpu(fn, rows)
-    fmt, P, page, c, dev = _pool(fn, rows, scales)
-    _need_ints(fn, "table", table, 2, dev)
-    S = _step(fn, dev, slots, cu_rows, first)
+    fmt, dev, P, page, c, n_slots, nbp, _, S = _step(fn, rows, scales, table, None, slots, cu_rows, first)
     if total < 0:
         _fail(fn, f"total={total} must be >= 0")
     tail = 0
@@ -230,7 +238,6 @@ def paged_read(rows, scales, table, slots, cu_rows, *, total, first=None, dtype=
     elif out.shape != (total, c) or out.get_device() != dev or not out.is_contiguous() or out.data_ptr() % 16:
         _fail(fn, f"out must be a contiguous, 16-byte aligned [{total}, {c}] tensor on {rows.device}")
     code = _lib.dtype_code(fn, out.dtype)
-    n_slots, nbp = table.shape
     _lib.call_on(dev, "kch_paged_read", rows.data_ptr(), _p(scales), table.data_ptr(), slots.data_ptr(),
                  cu_rows.data_ptr(), _p(first), out.data_ptr(), S, total, c, P, page, nbp, n_slots, tail, fmt,
                  code)

@@ -614,3 +614,40 @@ def test_operators_refuse(dev):
             app(**k)
     with pytest.raises(ValueError, match="total"):
         kch.paged_read(pool.rows, pool.scales, pool.blocks, s, cu, total=-1)
+
+
+def test_no_sequences_at_all(dev):
+    """S = 0: every row lies behind the last sequence; an empty pool is not read."""
+    import kch
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    rows = torch.zeros(0, 16, 64, device="cuda", dtype=torch.bfloat16)
+    q = torch.ones(3, 4, 64, device="cuda", dtype=torch.bfloat16)
+    out = kch.hca_paged_attention(q, rows, None, z(1, 1), z(1, 1), z(0), z(1), z(0), m2=8, sliding_window=8,
+                                  max_len=1, max_ctx=0)
+    assert (out == 0).all()
+    for dt in (torch.float32, torch.bfloat16):
+        assert (kch.paged_read(rows, None, z(1, 1), z(0), z(1), total=5, dtype=dt) == 0).all()
+    kch.hca_paged_append(q[:, 0], q[:, 0], torch.zeros(8, 64, device="cuda"), rows, None,
+                         torch.zeros(1, 3, 64, device="cuda"), z(1, 1), z(1, 1), z(0), z(1), z(0), m2=8, max_len=1)
+    with pytest.raises(RuntimeError, match="without pages"):
+        kch.hca_paged_attention(q, rows, None, z(1, 1), z(1, 1), z(1), z(2), z(1), m2=8, sliding_window=8, max_len=1)
+
+
+def test_chunks_longer_than_max_len(dev):
+    """max_len is a promise: what a chunk has past it is zeros (left as it was in out), the rest is right."""
+    rng = np.random.default_rng(21)
+    m2, win = 16, 16
+    for nh, lens in ((16, [5, 2]), (4, [40, 3])):
+        cut = 1 if nh == 16 else 20
+        pool = ref.Pool(2, *pages_for(lens, [100, 50], m2, win, 16), 16, 64, "e4m3")
+        fill(pool, lens, [100, 50], [0, 1], m2, win, rng)
+        q = torch.from_numpy(rng.standard_normal((sum(lens), nh, 64))).cuda().bfloat16()
+        whole = run_attention(pool, q, lens, [100, 50], [0, 1], m2, win, None, 8.0)
+        out = run_attention(pool, q, lens, [100, 50], [0, 1], m2, win, None, 8.0, max_len=cut)
+        got = torch.zeros(sum(lens), dtype=torch.bool)
+        got[:cut] = True
+        got[lens[0]:lens[0] + min(cut, lens[1])] = True
+        assert (out[~got] == 0).all() and (out[got].float() - whole[got].float()).abs().max() <= 2.0 ** -6
+        mine = torch.full_like(q, 9.0)
+        run_attention(pool, q, lens, [100, 50], [0, 1], m2, win, None, 8.0, max_len=cut, out=mine)
+        assert (mine[~got] == 9.0).all() and torch.equal(mine[got], out[got])
