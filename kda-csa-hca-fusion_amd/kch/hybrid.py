@@ -42,6 +42,8 @@ from .ops_csa import naive_csa
 from .ops_hca import naive_hca
 from .ops_kda import _recurrent_launch, kda_recurrent_into, naive_chunk_kda, naive_recurrent_kda
 from .ops_kda_backend import kda_forward, validate_kda_backend
+from .ops_w4 import linear_w4, quantize_w4
+from .paged import HCAPagedCache
 
 logger = logging.getLogger(__name__)
 
@@ -317,16 +319,19 @@ class _FusedWeightLayer(nn.Module):
         super().__init__()
         self._fused = _FusedWeight()
         self._fused_step = _FusedWeight()  # the decode step's operands
+        self._fused_w4 = {}  # group size -> the 4-bit copies of the projections
         self.register_load_state_dict_post_hook(_invalidate_after_load)
 
     def invalidate_weight_cache(self) -> None:
         """Drop the fused weight copies (call after writing parameters through ``.data``)."""
         self._fused.invalidate()
         self._fused_step.invalidate()
+        self._fused_w4.clear()
 
     def _apply(self, fn, *args, **kwargs):
         self._fused.invalidate()
         self._fused_step.invalidate()
+        self._fused_w4.clear()
         return super()._apply(fn, *args, **kwargs)
 
 
@@ -739,6 +744,50 @@ class HCAHybridLayer(_FusedWeightLayer):
                           dc=cfg.hca_dc, sliding_window=cfg.hca_sliding_window,
                           sink_logits=self.sink)
             return _out_proj(self.o_proj, o, residual), None
+
+    # ---- serving: sequences of unequal length over a paged cache ----
+    def paged_cache(self, n_pages: int, *, max_seqs: int, max_tokens: int, max_chunk: int = 1,
+                    page: int = 64, kv_dtype=torch.float8_e4m3fn) -> HCAPagedCache:
+        """A paged cache of this layer's sizes on its device."""
+        cfg = self.cfg
+        return HCAPagedCache(n_pages, cfg.hca_c, cfg.hca_m2, cfg.hca_sliding_window,
+                             max_seqs=max_seqs, max_tokens=max_tokens, max_chunk=max_chunk,
+                             page=page, kv_dtype=kv_dtype, device=self.W_KV.weight.device)
+
+    def forward_paged(self, x: torch.Tensor, cache: HCAPagedCache, slots, lens=None, *,
+                      residual: torch.Tensor | None = None, weight_group: int = 0):
+        """``[N, d]``: the layer's output for the next ``lens[i]`` tokens (1 each by default)
+        of the sequences ``slots`` of ``cache``, packed rows ``x`` ``[N, d]``; what ``forward``
+        gives at these positions of the whole sequences. ``residual`` is added.
+        ``weight_group`` 32, 64 or 128: the projections run on 4-bit copies of the weights
+        with groups of so many columns (bf16 or fp16 ``x``), made once. Forward only."""
+        cfg = self.cfg
+        c, nh, dc = cfg.hca_c, cfg.hca_nh, cfg.hca_dc
+        if x.dim() != 2 or x.shape[1] != cfg.d_model:
+            raise ValueError(f"forward_paged: x must be [N, {cfg.d_model}], got {tuple(x.shape)}")
+        proj = [self.W_KV.weight, self.W_Z.weight, self.W_DQ.weight]
+        with torch.no_grad():
+            if weight_group:
+                def build():
+                    ws = [torch.cat([p.detach() for p in proj], 0), self.W_UQ.weight, self.o_proj.weight]
+                    return [quantize_w4(w.to(x.device), weight_group, dtype=x.dtype) for w in ws]
+                fused = self._fused_w4.setdefault(weight_group, _FusedWeight())
+                w_in, w_up, w_out = fused.get(proj + [self.W_UQ.weight, self.o_proj.weight], x.dtype,
+                                              x.device, build)
+                C, Z, cQ = linear_w4(x, *w_in).split([c, c, dc], -1)
+                q = linear_w4(cQ, *w_up)
+            else:
+                C, Z, cQ = _linear(x, self._fused.get(proj, x.dtype, x.device)).split([c, c, dc], -1)
+                q = _linear(cQ, self.W_UQ.weight)
+            cache.append_step(slots, C, Z, self.B_pos, lens)
+            # q is L2-normalised in the kernel (F.normalize(q.float()) of the reference)
+            o = cache.forward_step(q.view(-1, nh, c), scale=1.0, sink_logits=self.sink, normalize_q=True)
+            o = o.reshape(-1, nh * c)
+            if weight_group:
+                return linear_w4(o, *w_out, residual=residual)
+            if residual is None:
+                return _linear(o, self.o_proj.weight)
+            return _linear_residual(o, self.o_proj.weight, residual)
 
 
 class HybridKCHAttention(nn.Module):
