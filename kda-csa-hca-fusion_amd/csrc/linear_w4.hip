@@ -105,12 +105,12 @@ __global__ __launch_bounds__(64 * KW) void linear_w4_kernel(LinearW4Params p) {
     const int k0 = 128 * pc;
 #pragma unroll
     for (int t = 0; t < NT; ++t) c.w[t] = wrow[t][TAIL && k0 + 32 * q >= K ? -q : 4 * pc];
-    const int ka = k0 + 8 * (lane & 7), kb = ka + 64;  // this lane's k of its two lines
-    const bool pa = TAIL && ka >= K, pb = TAIL && kb >= K;
-    c.x[0] = *reinterpret_cast<const uint4*>(xa + (pa ? 0 : k0));
-    c.x[1] = *reinterpret_cast<const uint4*>(xa + (pb ? 0 : k0 + 64));
-    c.x[2] = *reinterpret_cast<const uint4*>(xb + (pa ? 0 : k0));
-    c.x[3] = *reinterpret_cast<const uint4*>(xb + (pb ? 0 : k0 + 64));
+    const int kl = 8 * (lane & 7), ka = k0 + kl, kb = ka + 64;  // this lane's k of its two lines
+    const bool pa = TAIL && ka >= K, pb = TAIL && kb >= K;         // (past the row: its start instead)
+    c.x[0] = *reinterpret_cast<const uint4*>(xa + (pa ? -kl : k0));
+    c.x[1] = *reinterpret_cast<const uint4*>(xa + (pb ? -kl : k0 + 64));
+    c.x[2] = *reinterpret_cast<const uint4*>(xb + (pa ? -kl : k0));
+    c.x[3] = *reinterpret_cast<const uint4*>(xb + (pb ? -kl : k0 + 64));
     if (pa) c.x[0] = c.x[2] = make_uint4(0, 0, 0, 0);
     if (pb) c.x[1] = c.x[3] = make_uint4(0, 0, 0, 0);
 #pragma unroll

@@ -767,6 +767,7 @@ class HCAHybridLayer(_FusedWeightLayer):
             raise ValueError(f"forward_paged: x must be [N, {cfg.d_model}], got {tuple(x.shape)}")
         proj = [self.W_KV.weight, self.W_Z.weight, self.W_DQ.weight]
         with torch.no_grad():
+            w_in, w_up, B_pos, sink = self._step_weights(x.dtype, x.device)
             if weight_group:
                 def build():
                     ws = [torch.cat([p.detach() for p in proj], 0), self.W_UQ.weight, self.o_proj.weight]
@@ -777,11 +778,11 @@ class HCAHybridLayer(_FusedWeightLayer):
                 C, Z, cQ = linear_w4(x, *w_in).split([c, c, dc], -1)
                 q = linear_w4(cQ, *w_up)
             else:
-                C, Z, cQ = _linear(x, self._fused.get(proj, x.dtype, x.device)).split([c, c, dc], -1)
-                q = _linear(cQ, self.W_UQ.weight)
-            cache.append_step(slots, C, Z, self.B_pos, lens)
+                C, Z, cQ = _linear(x, w_in).split([c, c, dc], -1)
+                q = _linear(cQ, w_up)
+            cache.append_step(slots, C, Z, B_pos, lens)
             # q is L2-normalised in the kernel (F.normalize(q.float()) of the reference)
-            o = cache.forward_step(q.view(-1, nh, c), scale=1.0, sink_logits=self.sink, normalize_q=True)
+            o = cache.forward_step(q.view(-1, nh, c), scale=1.0, sink_logits=sink, normalize_q=True)
             o = o.reshape(-1, nh * c)
             if weight_group:
                 return linear_w4(o, *w_out, residual=residual)

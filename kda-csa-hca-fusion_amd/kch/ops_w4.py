@@ -49,6 +49,8 @@ def linear_w4(x, packed, scales, zeros=None, *, residual=None):
     if zeros is not None and (zeros.dtype is not torch.uint8 or zeros.shape != scales.shape
                               or not zeros.is_contiguous() or zeros.get_device() != dev):
         raise ValueError(f"{fn}: zeros must be a contiguous uint8 {tuple(scales.shape)} tensor on {x.device}")
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+        raise NotImplementedError(f"{fn}: no gradients (call it under torch.no_grad())")
     x2 = x if x.dim() == 2 else x.reshape(-1, K)
     M = x2.shape[0]
     ldx, one = x2.stride()

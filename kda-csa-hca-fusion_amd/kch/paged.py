@@ -28,7 +28,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops_csa import _HEAD_DIMS, _aligned, _f32_cached, _kernel_size, _pad_last
+from .ops_csa import _HEAD_DIMS, _aligned, _f32, _kernel_size, _pad_last
 
 _FORMATS = {torch.bfloat16: 0, torch.float8_e4m3fn: 1, torch.int8: 2}
 _I32 = torch.int32
@@ -108,6 +108,11 @@ def _step(fn, rows, scales, block_table, ring_table, slots, cu_seqlens, ctx_lens
     return fmt, dev, P, page, c, n_slots, nbp, nrp, S
 
 
+def _no_grad(fn, *ts):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        raise NotImplementedError(f"{fn}: no gradients (call it under torch.no_grad())")
+
+
 def _rows2d(x):
     """``x`` ``[N, c]`` with 16-byte aligned rows, and their stride."""
     ld, one = x.stride()
@@ -118,10 +123,11 @@ def _rows2d(x):
 
 
 def _f32_rows(t, dev):
-    """fp32, contiguous and 16-byte aligned on device ``dev``: ``t`` itself where it is."""
+    """fp32, contiguous and 16-byte aligned on device ``dev``: ``t`` itself where it is (a copy
+    is made on every call: keep such parameters in fp32)."""
     if t.dtype is torch.float32 and t.get_device() == dev and t.is_contiguous() and t.data_ptr() % 16 == 0:
         return t
-    return _aligned(_f32_cached(t, torch.device("cuda", dev)))
+    return _aligned(_f32(t, torch.device("cuda", dev)))
 
 
 def _p(t):
@@ -147,6 +153,7 @@ def hca_paged_append(C, Z, B_pos, rows, scales, state, block_table, ring_table, 
         _lib.require_gpu(fn, C, Z)
         _fail(fn, f"C and Z must be [N, {c}] of one dtype on {rows.device}, got {tuple(C.shape)} {C.dtype} and "
                   f"{tuple(Z.shape)} {Z.dtype}")
+    _no_grad(fn, C, Z)
     if m2 < 1:
         _fail(fn, f"m2={m2} must be >= 1")
     if B_pos.shape != (m2, c):
@@ -186,6 +193,7 @@ def hca_paged_attention(q, rows, scales, block_table, ring_table, slots, cu_seql
     if width != c or nh < 1 or q.get_device() != dev:
         _lib.require_gpu(fn, q)
         _fail(fn, f"q must be [N, nh, {c}] on {rows.device}, got {tuple(q.shape)} on {q.device}")
+    _no_grad(fn, q)
     code = _lib.dtype_code(fn, q.dtype)
     if m2 < 1:
         _fail(fn, f"m2={m2} must be >= 1")

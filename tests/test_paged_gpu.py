@@ -600,6 +600,10 @@ def test_operators_refuse(dev):
         attn(q=q.double())
     with pytest.raises(RuntimeError, match="GPU"):
         attn(q=q.cpu())
+    with pytest.raises(NotImplementedError, match="no gradients"):
+        attn(q=q.clone().requires_grad_())
+    with torch.no_grad():
+        attn(q=q.clone().requires_grad_())
 
     def app(**k):
         a = dict(C=C, Z=C, B_pos=Bp, rows=pool.rows, scales=pool.scales, state=pool.state, block_table=pool.blocks,
@@ -612,6 +616,8 @@ def test_operators_refuse(dev):
                    (dict(state=pool.state[:, :2]), "state")):
         with pytest.raises(ValueError, match=msg):
             app(**k)
+    with pytest.raises(NotImplementedError, match="no gradients"):
+        app(Z=C.clone().requires_grad_())
     with pytest.raises(ValueError, match="total"):
         kch.paged_read(pool.rows, pool.scales, pool.blocks, s, cu, total=-1)
 

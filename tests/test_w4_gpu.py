@@ -164,6 +164,8 @@ def test_refusals(dev):
             kch.linear_w4(*args)
     with pytest.raises(ValueError, match="residual"):
         kch.linear_w4(x, packed, scales, zeros, residual=x)
+    with pytest.raises(NotImplementedError, match="no gradients"):
+        kch.linear_w4(x.clone().requires_grad_(), packed, scales, zeros)
     with pytest.raises(RuntimeError, match="GPU"):
         kch.linear_w4(x.cpu(), packed, scales, zeros)
     for w, g, msg in ((x, 48, "group_size"), (x[:, :100], 64, "group_size"), (x[0], 64, "weight")):
