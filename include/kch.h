@@ -573,7 +573,8 @@ int kch_linear_up(const void* x, long long ldx, const void* w, long long ldw, vo
  * replayed with new contents. Sequences that they do not describe rightly
  * (rows outside 0 .. N - 1, a slot outside the tables, a negative position)
  * are passed over. A table entry that names no page of the pool reads as a row of
- * zeros and is not written. max_len is at least the longest chunk.
+ * zeros and is not written. max_len is at least the longest chunk (the attention
+ * leaves a longer one's rows past it as they were, or zeros with zero_tail).
  */
 
 /*

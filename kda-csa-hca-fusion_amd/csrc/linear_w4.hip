@@ -72,7 +72,7 @@ template <int NT, int G> struct W4Piece {
 // bound the kernel (16 rows, N 4096, K 8192: 13.7 against 10.1 us). VEC: N is a multiple of 4,
 // four scales are one load. The loop has no load behind a branch: a wait there would drain
 // every load in flight (the same kernel with such loads took 145 us where it took 43).
-// At 16 rows, N 16384, K 8192 20 us, 3.5 TB/s; 13.8 us is what its 71 MB take at the rate of a
+// At 16 rows, N 16384, K 8192 18.6 us, 3.8 TB/s; 13.9 us is what its 71 MB take at the rate of a
 // large copy. Past the stream it is the 56 vector instructions a tile and 128 k, mostly the
 // codes' unpacking.
 template <typename T, int NT, int KW, int G, bool ZP, bool VEC, bool KT>

@@ -7,8 +7,10 @@
 // and 0 where no key is visible (/root/reference/ops_hca.py:132-194 over a cache,
 // /root/reference/ops_decoding_cache.py:1268-1395; chunks of one token are its
 // decode step). The query is rounded to bf16 and so are the weights e^(s - M) in
-// the second product, whose factors the matrix instruction takes in bf16; keys
-// are exact in bf16 in every storage format, scores, sums and outputs are fp32.
+// the second product: bf16 because it has the range of fp32, which unnormalised
+// queries and rows scaled by any power of two need (fp16, finer by three bits, has
+// not), and because keys are exact in it in every storage format. Scores, sums and
+// outputs are fp32.
 //
 // All heads share the keys (MQA), so the query rows of a sequence are its tokens
 // times its heads, nh rows a token, and a 16-row MFMA tile may hold rows of
@@ -18,8 +20,8 @@
 // bf16 once on their way into LDS for all of the workgroup's rows
 // (paged_attn_kernel). Where a sequence has few rows (one token of 16 heads is one
 // group) the call is bound by the rows' bytes, and the waves of a workgroup split
-// the keys: each takes 32-key steps of its own through its own LDS, two of them in
-// flight, without a barrier, and the waves' sums are joined at the end
+// the keys: each takes 32-key steps of its own through its own LDS, one in flight
+// beside the one in LDS, without a barrier, and the waves' sums are joined at the end
 // (paged_token_kernel). Long contexts are cut into ranges of keys, one workgroup
 // each, whose partial sums a second kernel joins, so that a few sequences fill the
 // device.
@@ -28,6 +30,16 @@
 // sits in LDS as zeros beside a NaN that is added to its scores: rows that do
 // not see it stay as they are (0 times NaN would reach them in the second
 // product), rows that do become NaN.
+//
+// Measured (16 heads of 128, e4m3 rows, blocks of 128 tokens, a window of 128):
+//   one token for each of 128 contexts of 512K to 1M tokens  28.9 us + 4.9 the join, for
+//     99.6 MB 3.4 TB/s (a large copy 5.1): bound by the rows' bytes, and by ranges that
+//     end at different times
+//   one token behind 5003, 51 KB  9.7 us: latencies one after another (the step's
+//     arrays, page entries, rows, the waves' join)
+//   up to 2048 tokens behind 64K to 128K in each of 8 sequences  125 us, 565 TFLOP/s: the
+//     issue of vector instructions beside the products (71 a 16 products, most of them
+//     the softmax; products busy for 38% of the cycles)
 
 #include "paged.h"
 
@@ -117,7 +129,7 @@ __device__ __forceinline__ void store_group(const PagedAttnParams& p, const MqaW
 // in turn. BIG: pages of at least 32 rows (one table entry a step). No load is behind a
 // branch (a wait there would drain every load in flight): past the end the last
 // step is read again.
-// Workgroups a CU at least (what keeps two steps in registers without spilling).
+// Workgroups a CU at least (as many as leave registers for a step in flight without spilling).
 constexpr int token_min_blocks(int HD, int FMT, int QW) {
   return (QW == 1 ? 3 : 2) - (HD == 128 && FMT == PF_BF16 ? 1 : 0);
 }
@@ -420,7 +432,10 @@ __device__ __forceinline__ RowKeys row_keys(const PagedAttnParams& p, const Page
 
 // RG groups of 16 rows of a sequence, QW of them a wave, and a range of keys. Two
 // workgroups of 8 waves a CU (128 registers): 132 us where one took 156, for 8 chunks of up
-// to 2048 tokens behind 128K.
+// to 2048 tokens behind 128K. Two groups a wave on half as many waves, with the next
+// step's scores between this one's softmax, halve the LDS reads and nearly the vector
+// instructions, but two waves a SIMD wait for LDS: 122 us there, and 76 where this
+// takes 71 for 16 chunks without a context, 167 where it takes 143 on bf16 rows.
 template <int HD, int FMT, int RG, int QW, typename T>
 __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_kernel(PagedAttnParams p) {
   using W = MqaWave<HD>;

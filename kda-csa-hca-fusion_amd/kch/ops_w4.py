@@ -49,7 +49,8 @@ def linear_w4(x, packed, scales, zeros=None, *, residual=None):
     if zeros is not None and (zeros.dtype is not torch.uint8 or zeros.shape != scales.shape
                               or not zeros.is_contiguous() or zeros.get_device() != dev):
         raise ValueError(f"{fn}: zeros must be a contiguous uint8 {tuple(scales.shape)} tensor on {x.device}")
-    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+    if torch.is_grad_enabled() and (x.requires_grad or scales.requires_grad
+                                    or (residual is not None and residual.requires_grad)):
         raise NotImplementedError(f"{fn}: no gradients (call it under torch.no_grad())")
     x2 = x if x.dim() == 2 else x.reshape(-1, K)
     M = x2.shape[0]
@@ -95,7 +96,7 @@ def quantize_w4(weight, group_size=128, *, zero_points=True, dtype=None):
         dtype = weight.dtype if weight.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
     if dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"{fn}: scales are bfloat16 or float16, got {dtype}")
-    w = weight.detach().float().view(N, K // group_size, group_size)
+    w = weight.detach().float().reshape(N, K // group_size, group_size)
     if zero_points:
         lo, hi = w.amin(-1).clamp_max(0.0), w.amax(-1).clamp_min(0.0)
         s = ((hi - lo) / 15).to(dtype)

@@ -109,7 +109,7 @@ def _step(fn, rows, scales, block_table, ring_table, slots, cu_seqlens, ctx_lens
 
 
 def _no_grad(fn, *ts):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
         raise NotImplementedError(f"{fn}: no gradients (call it under torch.no_grad())")
 
 
@@ -153,7 +153,7 @@ def hca_paged_append(C, Z, B_pos, rows, scales, state, block_table, ring_table, 
         _lib.require_gpu(fn, C, Z)
         _fail(fn, f"C and Z must be [N, {c}] of one dtype on {rows.device}, got {tuple(C.shape)} {C.dtype} and "
                   f"{tuple(Z.shape)} {Z.dtype}")
-    _no_grad(fn, C, Z)
+    _no_grad(fn, C, Z, B_pos)
     if m2 < 1:
         _fail(fn, f"m2={m2} must be >= 1")
     if B_pos.shape != (m2, c):
@@ -183,7 +183,8 @@ def hca_paged_attention(q, rows, scales, block_table, ring_table, slots, cu_seql
     ``max(0, p - sliding_window + 1) .. p`` in one softmax with the sink; 0 where it
     sees none. ``max_len`` is at least the longest chunk, ``max_ctx`` at least the largest
     of ``ctx_lens`` (it lays the work out). Returns ``[N, nh, c]`` in ``q.dtype``, or
-    writes ``out``; rows behind the last sequence are zeros, in ``out`` as they were.
+    writes ``out``; rows behind the last sequence, and of a longer chunk past ``max_len``,
+    are zeros, in ``out`` as they were.
     The products are bf16 with fp32 sums whatever ``q``'s type.
     """
     fn = "hca_paged_attention"
@@ -193,7 +194,7 @@ def hca_paged_attention(q, rows, scales, block_table, ring_table, slots, cu_seql
     if width != c or nh < 1 or q.get_device() != dev:
         _lib.require_gpu(fn, q)
         _fail(fn, f"q must be [N, nh, {c}] on {rows.device}, got {tuple(q.shape)} on {q.device}")
-    _no_grad(fn, q)
+    _no_grad(fn, q, sink_logits)
     code = _lib.dtype_code(fn, q.dtype)
     if m2 < 1:
         _fail(fn, f"m2={m2} must be >= 1")
@@ -259,7 +260,9 @@ class HCAPagedCache:
     new tokens of some sequences, ``forward_step`` their queries, ``release`` gives a
     sequence's pages back. ``max_tokens`` bounds a sequence's length, ``max_chunk``
     the tokens a step takes of one. Widths between the kernels' own are held
-    zero-padded. A single-threaded object on one stream, as the other caches.
+    zero-padded. A single-threaded object on one stream, as the other caches; its steps'
+    counts come from the host, so they cannot be captured into a graph (the operators
+    over the same tensors can).
     """
 
     def __init__(self, n_pages, c, m2, win, *, max_seqs, max_tokens, max_chunk=1, page=64,
@@ -316,6 +319,11 @@ class HCAPagedCache:
             _fail(f"HCAPagedCache.{fn}", f"slot {slot!r} holds no sequence")
         return slot
 
+    def _eager(self, fn):
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"HCAPagedCache.{fn}: a graph would replay this step's counts; capture the operators "
+                               f"hca_paged_append, hca_paged_attention and paged_read instead")
+
     def _upload(self, *lists):
         """int32 lists on the device, in one copy."""
         flat = [v for x in lists for v in x]
@@ -329,6 +337,7 @@ class HCAPagedCache:
 
     def add(self) -> int:
         """Opens a sequence and returns its slot."""
+        self._eager("add")
         if not self._free_slots:
             raise RuntimeError("HCAPagedCache.add: every slot holds a sequence")
         ring = self._take("add", 0 if self.ring_table is None else self.ring_table.shape[1])
@@ -352,6 +361,7 @@ class HCAPagedCache:
         """Appends ``lens[i]`` tokens (1 each by default) to sequence ``slots[i]``:
         ``C_new, Z_new`` ``[sum(lens), c]``, packed in that order."""
         fn = "append_step"
+        self._eager(fn)
         slots = list(slots)
         lens = [1] * len(slots) if lens is None else list(lens)
         if len(lens) != len(slots) or len(set(slots)) != len(slots):
@@ -400,6 +410,7 @@ class HCAPagedCache:
     def forward_step(self, q, *, scale=None, sink_logits=None, normalize_q=None):
         """``[N, nh, c]`` in ``q.dtype``: the queries of the last ``append_step``'s tokens."""
         fn = "HCAPagedCache.forward_step"
+        self._eager("forward_step")
         if self._last is None:
             _fail(fn, "append_step first")
         _, slots, cu, ctx, n, max_len, max_ctx = self._last
@@ -417,6 +428,7 @@ class HCAPagedCache:
 
     def read_blocks(self, slot, dtype=torch.bfloat16):
         """The compressed rows ``[n_blocks, c]`` of a sequence."""
+        self._eager("read_blocks")
         n = self.n_blocks(self._slot("read_blocks", slot))
         s, cu = self._upload([slot], [0, n])
         out = paged_read(self.rows, self.scales, self.block_table, s, cu, total=n, dtype=dtype)
@@ -424,6 +436,7 @@ class HCAPagedCache:
 
     def read_window(self, slot, dtype=torch.bfloat16):
         """The window rows ``[min(win, tokens), c]`` of a sequence, oldest first."""
+        self._eager("read_window")
         t = self.n_tokens(slot)
         n = min(self.win, t)
         if not n:

@@ -657,3 +657,38 @@ def test_chunks_longer_than_max_len(dev):
         mine = torch.full_like(q, 9.0)
         run_attention(pool, q, lens, [100, 50], [0, 1], m2, win, None, 8.0, max_len=cut, out=mine)
         assert (mine[~got] == 9.0).all() and torch.equal(mine[got], out[got])
+
+
+def test_parameters_that_ask_for_gradients_are_refused(dev):
+    import kch
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    rows = torch.zeros(2, 16, 64, device="cuda", dtype=torch.bfloat16)
+    x = torch.ones(1, 64, device="cuda", dtype=torch.bfloat16)
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    at = (z(1, 1), torch.ones(1, 1, dtype=torch.int32, device="cuda"), z(1), cu, z(1))
+    with pytest.raises(NotImplementedError, match="no gradients"):
+        kch.hca_paged_append(x, x, torch.zeros(8, 64, device="cuda", requires_grad=True), rows, None,
+                             torch.zeros(1, 3, 64, device="cuda"), *at, m2=8, max_len=1)
+    with pytest.raises(NotImplementedError, match="no gradients"):
+        kch.hca_paged_attention(x[:, None], rows, None, *at, m2=8, sliding_window=8, max_len=1,
+                                sink_logits=torch.zeros(1, device="cuda", requires_grad=True))
+
+
+def test_cache_refuses_capture(dev, monkeypatch):
+    """The cache's counts come from the host: a graph would replay this step's."""
+    import kch
+    cache = kch.HCAPagedCache(4, 64, 8, 8, max_seqs=2, max_tokens=64, page=16)
+    s = cache.add()
+    x = torch.ones(1, 64, device="cuda", dtype=torch.bfloat16)
+    Bp = torch.zeros(8, 64, device="cuda")
+    cache.append_step([s], x, x, Bp)
+    out = cache.forward_step(x[:, None])
+    free, n = cache.n_free_pages, cache.n_tokens(s)
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        for f in (cache.add, lambda: cache.append_step([s], x, x, Bp), lambda: cache.forward_step(x[:, None]),
+                  lambda: cache.read_blocks(s), lambda: cache.read_window(s)):
+            with pytest.raises(RuntimeError, match="graph"):
+                f()
+    assert cache.n_free_pages == free and cache.n_tokens(s) == n
+    assert torch.equal(cache.forward_step(x[:, None]), out)

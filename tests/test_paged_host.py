@@ -173,3 +173,11 @@ def test_references_agree_with_the_oracle():
     whole = ref.append(Cn, Zn, Bp, [T + 2], [0], [0], np.zeros((1, 3, c)), m2=m2)[0]
     assert np.abs(more[0, T // m2] - whole[0, T // m2]).max() < 1e-12
     assert ctypes.sizeof(ctypes.c_void_p) == 8
+
+
+def test_quantize_w4_of_a_transposed_weight():
+    import kch
+    torch.manual_seed(1)
+    w = torch.randn(128, 24)
+    for a, b in zip(kch.quantize_w4(w.t(), 32), kch.quantize_w4(w.t().contiguous(), 32)):
+        assert torch.equal(a, b)

@@ -173,3 +173,11 @@ def test_refusals(dev):
             kch.quantize_w4(w, g)
     with pytest.raises(ValueError, match="bias"):
         kch.W4Linear.from_linear(torch.nn.Linear(64, 8))
+
+
+def test_scales_that_ask_for_gradients_are_refused(dev):
+    import kch
+    packed, scales, zeros = make(32, 128, 64, True, "bf16", 3)
+    x = torch.zeros(2, 128, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(NotImplementedError, match="no gradients"):
+        kch.linear_w4(x, packed, scales.clone().requires_grad_(), zeros)
