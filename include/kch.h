@@ -605,6 +605,8 @@ int kch_hca_paged_append(const void* C, long long ldc, const void* Z, long long 
  * q, out [N, nh, c] of dtype (contiguous, 16-byte aligned), sink [nh] fp32 or
  * NULL; normalize_q: L2-normalise the queries. max_ctx is at least the largest
  * ctx (it lays the work out; a larger one is answered rightly, if slower).
+ * The products take bf16, with dtype fp16 fp16: rows with values past its range
+ * then read as NaN (kept in 8 bits, past four times its range).
  * Rows of out that belong to no sequence behind cu[S] are left as they were, or
  * zeros with zero_tail. ws as kch_hca_paged_attn_ws_bytes says, 256-byte aligned.
  */

@@ -198,14 +198,30 @@ __device__ __forceinline__ void store_rows(const f32x4 (&o)[HD / 16], float f, O
   }
 }
 
-// One wave, one query, up to 16 heads of head dim HD (64 or 128).
-template <int HD>
+// The 16-bit types of the matrix products.
+template <typename E> struct Mfma16;
+template <> struct Mfma16<bf16_t> {
+  typedef bf16x8 v8;
+  static __device__ __forceinline__ f32x4 run(v8 a, v8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct Mfma16<_Float16> {
+  typedef f16x8 v8;
+  static __device__ __forceinline__ f32x4 run(v8 a, v8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+// One wave, one query, up to 16 heads of head dim HD (64 or 128). E: the products' type.
+template <int HD, typename E = bf16_t>
 struct MqaWave {
+  typedef typename Mfma16<E>::v8 v8;
   static constexpr int NS = HD / 32;          // 32-wide k steps of S^T
   static constexpr int NT = HD / 16;          // O^T tiles
   static constexpr int STAGE_ELEMS = 32 * HD;  // bf16 of a 32-row stage (chunk2)
 
-  bf16x8 qf[NS];  // Q fragments: head n, dims 8q + 32s (sign of the scale folded in)
+  v8 qf[NS];  // Q fragments: head n, dims 8q + 32s (sign of the scale folded in)
   f32x4 o[NT];
   float M;        // softmax reference point of head n (log2 units), finite
   float L;        // sum of p over this lane's keys (finalize(): over the head)
@@ -255,7 +271,8 @@ struct MqaWave {
     for (int s = 0; s < NS; ++s) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[s][i] *= inv;
-      qf[s] = to_bf16x8(f[s]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) qf[s][i] = (E)f[s][i];
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -266,17 +283,17 @@ struct MqaWave {
   }
 
   // S^T accumulator of 16 key rows whose fragments are k (row n of the lane).
-  __device__ __forceinline__ f32x4 scores(const bf16x8 (&k)[NS]) const {
+  __device__ __forceinline__ f32x4 scores(const v8 (&k)[NS]) const {
     f32x4 st = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < NS; ++s) st = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[s], qf[s], st, 0, 0, 0);
+    for (int s = 0; s < NS; ++s) st = Mfma16<E>::run(k[s], qf[s], st);
     return st;
   }
 
   // Softmax step over 32 keys: sc = this lane's raw scores of keys 4q..4q+3
   // and 16+4q..16+4q+3 (-inf = masked). Rescales o and L when a score moves
   // M, adds the keys' p to L and returns p as the B operand of the O^T update.
-  __device__ __forceinline__ bf16x8 softmax32(const float (&sc)[8]) {
+  __device__ __forceinline__ v8 softmax32(const float (&sc)[8]) {
     bool up = false;
 #pragma unroll
     for (int e = 0; e < 8; ++e) up |= sc[e] > thr;
@@ -298,13 +315,13 @@ struct MqaWave {
 #pragma unroll
     for (int e = 0; e < 8; ++e) pe[e] = fast_exp2(fmaf(sc[e], qscale2, nm));
     L += ((pe[0] + pe[1]) + (pe[2] + pe[3])) + ((pe[4] + pe[5]) + (pe[6] + pe[7]));
-    return __builtin_convertvector(pe, bf16x8);
+    return __builtin_convertvector(pe, v8);
   }
 
   // V^T fragment t (16 dims x 32 keys) of 32 key rows in a swizzled LDS tile:
   // column 16t + n of rows 4q .. 4q + 3 of each 16-row slice, one transposing
   // read per slice.
-  __device__ __forceinline__ static bf16x8 vt_frag(const bf16_t* rows, const TileOffsets<HD>& to,
+  __device__ __forceinline__ static v8 vt_frag(const E* rows, const TileOffsets<HD>& to,
                                                    int t) {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     const int vo = to.vt(t);
@@ -312,7 +329,7 @@ struct MqaWave {
         (__attribute__((address_space(3))) s16x4*)(rows + vo));
     const s16x4 r1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
         (__attribute__((address_space(3))) s16x4*)(rows + 16 * HD + vo));
-    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(r0, r1, 0, 1, 2, 3, 4, 5, 6, 7));
+    return __builtin_bit_cast(v8, __builtin_shufflevector(r0, r1, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 
   // Softmax step and O^T update over 32 keys whose rows (the V^T source) are

@@ -68,20 +68,53 @@ __device__ __forceinline__ float row_scale(int code) {
   return __uint_as_float(code == kScaleNan ? 0x7fc00000u : (uint32_t)code << 23);
 }
 
-// Four codes as bf16 values (exact).
-template <int FMT>
-__device__ __forceinline__ uint2 dequant4_bf16(uint32_t w, float scale) {
-  typedef bf16_t bf16x2 __attribute__((ext_vector_type(2)));
+// Rows as the operands of the attention's products, bf16 or fp16 (E). In fp16 the
+// 8-bit formats' values are held as a quarter: their largest may be rounded up past fp16's
+// (65504 to 65536), and at a quarter every row of values of fp16 fits. `top`: codes
+// of larger scales, and bf16 values of larger magnitude (past 65536, itself taken as
+// 65504), are rows beyond that, which read as NaN.
+template <int FMT, typename E> struct PagedKey {
+  static constexpr float held = 1.f;
+  static constexpr int top = FMT == PF_BF16 ? 0x7f7f : kScaleNan - 1;
+};
+template <int FMT> struct PagedKey<FMT, _Float16> {
+  static constexpr float held = FMT == PF_BF16 ? 1.f : 0.25f;
+  static constexpr int top = FMT == PF_BF16 ? 0x4780 : FMT == PF_E4M3 ? 127 + 9 : 127 + 11;
+};
+
+// Four codes as values (exact in bf16, and in fp16 down to its least steps).
+template <int FMT, typename E>
+__device__ __forceinline__ uint2 dequant4(uint32_t w, float scale) {
+  typedef E ex2 __attribute__((ext_vector_type(2)));
+  typedef E ex4 __attribute__((ext_vector_type(4)));
   if constexpr (FMT == PF_E4M3) {
-    const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false);
-    const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true);
+    ex2 lo, hi;
+    if constexpr (__is_same(E, _Float16)) {
+      lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, false);
+      hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true);
+    } else {
+      lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false);
+      hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true);
+    }
     return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
   } else {
-    bf16x4 r;
+    ex4 r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = (bf16_t)((float)(int8_t)(w >> (8 * i)) * scale);
+    for (int i = 0; i < 4; ++i) r[i] = (E)((float)(int8_t)(w >> (8 * i)) * scale);
     return __builtin_bit_cast(uint2, r);
   }
+}
+// Two bf16 values of a word as two of E (fp16: towards zero, which only values below
+// its normal range meet, and 65536).
+template <typename E> __device__ __forceinline__ uint32_t bf16_pair(uint32_t w) {
+  if constexpr (__is_same(E, _Float16))
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(w << 16),
+                                                                   __uint_as_float(w & 0xffff0000u)));
+  else
+    return w;
+}
+template <typename E> __device__ __forceinline__ uint4 bf16_pairs(uint4 v) {
+  return make_uint4(bf16_pair<E>(v.x), bf16_pair<E>(v.y), bf16_pair<E>(v.z), bf16_pair<E>(v.w));
 }
 
 // A sequence of the step: its slot, first row and length (0 where the arrays do

@@ -6,11 +6,14 @@
 //   s = scale q^ K^T,  out = sum_k e^(s_k) K_k / (sum_k e^(s_k) + e^sink_h)
 // and 0 where no key is visible (/root/reference/ops_hca.py:132-194 over a cache,
 // /root/reference/ops_decoding_cache.py:1268-1395; chunks of one token are its
-// decode step). The query is rounded to bf16 and so are the weights e^(s - M) in
-// the second product: bf16 because it has the range of fp32, which unnormalised
-// queries and rows scaled by any power of two need (fp16, finer by three bits, has
-// not), and because keys are exact in it in every storage format. Scores, sums and
-// outputs are fp32.
+// decode step). The query is rounded to 16 bits and so are the weights e^(s - M) in
+// the second product: to bf16, which has the range of fp32 that unnormalised queries
+// and rows scaled by any power of two need and holds the rows of every storage
+// format exactly; to fp16, finer by three bits, where the queries are fp16, for what
+// such a model's rows are fits it (paged.h). Scores, sums and outputs are fp32. The
+// second rounding of a bf16 query by itself is what leaves a bf16 output 0.0025
+// off where its own rounding leaves 0.0017 (both products in two parts would take the
+// tile kernel's issue time up by 40%).
 //
 // All heads share the keys (MQA), so the query rows of a sequence are its tokens
 // times its heads, nh rows a token, and a 16-row MFMA tile may hold rows of
@@ -107,18 +110,23 @@ __device__ __forceinline__ int computed_rows(const PagedAttnParams& p, const Pag
   return min(sq.len, p.max_len) * p.nh;  // N nh is below 2^30
 }
 
+// The type of the products for queries of type T.
+template <typename T> struct Prod { typedef bf16_t type; };
+template <> struct Prod<_Float16> { typedef _Float16 type; };
+
 // One 16-row group's output, or its partial sums for the join of its ranges.
-template <int HD, typename T>
-__device__ __forceinline__ void store_group(const PagedAttnParams& p, const MqaWave<HD>& w, long long g, int live,
+template <int HD, int FMT, typename T, typename E>
+__device__ __forceinline__ void store_group(const PagedAttnParams& p, const MqaWave<HD, E>& w, long long g, int live,
                                             bool whole, int head, void* stage) {
+  constexpr float unit = 1.f / PagedKey<FMT, E>::held;
   if (whole) {
-    const float f = w.finish(p.sink != nullptr, p.sink ? p.sink[head] : 0.f);
+    const float f = unit * w.finish(p.sink != nullptr, p.sink ? p.sink[head] : 0.f);
     store_rows<HD, T>(w.o, f, static_cast<T*>(p.out) + g * HD, live, stage);
     return;
   }
   const int n = lane_id() & 15;
   const long long gp = (long long)blockIdx.z * p.pool.N * p.nh + g;
-  store_rows<HD, float>(w.o, 1.f, p.part_o + gp * HD, live, stage);
+  store_rows<HD, float>(w.o, unit, p.part_o + gp * HD, live, stage);
   if (lane_id() < 16 && n < live) {
     p.part_ml[2 * (gp + n)] = w.M;
     p.part_ml[2 * (gp + n) + 1] = w.L;
@@ -135,13 +143,16 @@ constexpr int token_min_blocks(int HD, int FMT, int QW) {
 }
 template <int HD, int FMT, int QW, bool BIG, typename T>
 __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_token_kernel(PagedAttnParams p) {
-  using W = MqaWave<HD>;
+  typedef typename Prod<T>::type E;
+  typedef PagedKey<FMT, E> Key;
+  using W = MqaWave<HD, E>;
+  typedef typename W::v8 v8;
   constexpr int ROWB = FMT == PF_BF16 ? 2 * HD : HD;  // bytes of a key row
   constexpr int TPR = ROWB / 16;                      // lanes per key row
   constexpr int RPI = 64 / TPR;                       // key rows of a load
   constexpr int NLI = 32 / RPI;                       // loads of a step
   constexpr int NP = BIG ? 1 : NLI;                   // table entries of a lane
-  __shared__ __attribute__((aligned(16))) bf16_t stage_all[4][32 * HD];
+  __shared__ __attribute__((aligned(16))) E stage_all[4][32 * HD];
   __shared__ float ml[4][16][2];
   __shared__ float poison[4][32];
   const PagedPool& pl = p.pool;
@@ -155,7 +166,7 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
   const int lrow = lane / TPR, lch = lane % TPR;
   const uint32_t cap = (uint32_t)pl.nrp << pl.log2page;
   const uint32_t lmask = (1u << pl.log2page) - 1;
-  bf16_t* const stage = stage_all[wv];
+  E* const stage = stage_all[wv];
   const TileOffsets<HD> to;
 
   const int r0 = blockIdx.x * 16 * QW;
@@ -252,7 +263,7 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
       const int tok = rr / p.nh;
       head[u] = rr - tok * p.nh;
       w[u].template init_always<T>(static_cast<const T*>(p.q) + ((long long)sq.row0 * p.nh + rr) * HD, live,
-                                   p.normalize_q != 0, p.scale);
+                                   p.normalize_q != 0, p.scale / Key::held);
       const uint32_t pos = sq.ctx + tok;
       const uint32_t f = pos + 1 > (uint32_t)p.win ? pos + 1 - p.win : 0;
       // (a padding row is never stored: it masks nothing)
@@ -285,9 +296,9 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
           const uint32_t x[4] = {s.v[i].x, s.v[i].y, s.v[i].z, s.v[i].w};
           bad[i] = false;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) bad[i] |= (x[e] & 0x7f80u) == 0x7f80u || (x[e] & 0x7f800000u) == 0x7f800000u;
+          for (int e = 0; e < 4; ++e) bad[i] |= (x[e] & 0x7fffu) > Key::top || (x[e] >> 16 & 0x7fffu) > Key::top;
         } else {
-          bad[i] = s.code[i] == kScaleNan;
+          bad[i] = s.code[i] > Key::top;
         }
         some |= bad[i];
       }
@@ -305,14 +316,14 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
 #pragma unroll
       for (int i = 0; i < NLI; ++i) {
         const uint32_t row = step_row(i);
-        bf16_t* const dst = stage + row * HD;
+        E* const dst = stage + row * HD;
         const int sw = tile_swz<HD>(row & 15);
         if constexpr (FMT == PF_BF16) {
-          *reinterpret_cast<uint4*>(dst + 8 * (lch ^ sw)) = s.v[i];
+          *reinterpret_cast<uint4*>(dst + 8 * (lch ^ sw)) = bf16_pairs<E>(s.v[i]);
         } else {
-          const float sc = __uint_as_float((uint32_t)s.code[i] << 23);
-          const uint2 a = dequant4_bf16<FMT>(s.v[i].x, sc), c = dequant4_bf16<FMT>(s.v[i].y, sc);
-          const uint2 d = dequant4_bf16<FMT>(s.v[i].z, sc), e = dequant4_bf16<FMT>(s.v[i].w, sc);
+          const float sc = Key::held * __uint_as_float((uint32_t)s.code[i] << 23);
+          const uint2 a = dequant4<FMT, E>(s.v[i].x, sc), c = dequant4<FMT, E>(s.v[i].y, sc);
+          const uint2 d = dequant4<FMT, E>(s.v[i].z, sc), e = dequant4<FMT, E>(s.v[i].w, sc);
           *reinterpret_cast<uint4*>(dst + 8 * ((2 * lch) ^ sw)) = make_uint4(a.x, a.y, c.x, c.y);
           *reinterpret_cast<uint4*>(dst + 8 * ((2 * lch + 1) ^ sw)) = make_uint4(d.x, d.y, e.x, e.y);
         }
@@ -326,16 +337,16 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
       f32x4 ra[QW], rb[QW];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        bf16x8 kf[W::NS];
+        v8 kf[W::NS];
 #pragma unroll
-        for (int e = 0; e < W::NS; ++e) kf[e] = *reinterpret_cast<const bf16x8*>(stage + 16 * HD * h + to.key(e));
+        for (int e = 0; e < W::NS; ++e) kf[e] = *reinterpret_cast<const v8*>(stage + 16 * HD * h + to.key(e));
 #pragma unroll
         for (int u = 0; u < QW; ++u) {
           if (h == 0) ra[u] = w[u].scores(kf);
           else rb[u] = w[u].scores(kf);
         }
       }
-      bf16x8 pb8[QW];
+      v8 pb8[QW];
 #pragma unroll
       for (int u = 0; u < QW; ++u) {
         float sc[8] = {ra[u][0], ra[u][1], ra[u][2], ra[u][3], rb[u][0], rb[u][1], rb[u][2], rb[u][3]};
@@ -355,10 +366,10 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
       }
 #pragma unroll
       for (int t = 0; t < W::NT; ++t) {
-        const bf16x8 va = W::vt_frag(stage, to, t);
+        const v8 va = W::vt_frag(stage, to, t);
 #pragma unroll
         for (int u = 0; u < QW; ++u)
-          w[u].o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb8[u], w[u].o[t], 0, 0, 0);
+          w[u].o[t] = Mfma16<E>::run(va, pb8[u], w[u].o[t]);
       }
     };
 
@@ -411,7 +422,7 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
     __syncthreads();  // the sums are read before their place is staged over
     const int r = r0 + 16 * u;
     if (wv == u % 4 && r < nrow)
-      store_group<HD, T>(p, w[u], (long long)sq.row0 * p.nh + r, min(16, nrow - r), whole, head[u], ob);
+      store_group<HD, FMT, T>(p, w[u], (long long)sq.row0 * p.nh + r, min(16, nrow - r), whole, head[u], ob);
   }
 }
 
@@ -438,7 +449,10 @@ __device__ __forceinline__ RowKeys row_keys(const PagedAttnParams& p, const Page
 // takes 71 for 16 chunks without a context, 167 where it takes 143 on bf16 rows.
 template <int HD, int FMT, int RG, int QW, typename T>
 __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_kernel(PagedAttnParams p) {
-  using W = MqaWave<HD>;
+  typedef typename Prod<T>::type E;
+  typedef PagedKey<FMT, E> Key;
+  using W = MqaWave<HD, E>;
+  typedef typename W::v8 v8;
   constexpr int NWV = RG / QW, NTH = 64 * NWV;
   constexpr int ROWS = 16 * RG;
   constexpr int EPL = FMT == PF_BF16 ? 8 : 16;  // row elements of a lane's 16 bytes
@@ -446,7 +460,7 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
   constexpr int RSTEP = NTH / TPR;              // key rows of a load instruction of the workgroup
   constexpr int NLD = KC / RSTEP;
   static_assert(NLD >= 1 && KC % RSTEP == 0 && RSTEP % 16 == 0, "tile loads");
-  __shared__ __attribute__((aligned(16))) bf16_t tile[2][KC * HD];
+  __shared__ __attribute__((aligned(16))) E tile[2][KC * HD];
   __shared__ __attribute__((aligned(16))) float poison[2][KC];
   __shared__ int any_bad;  // some row so far is not finite
 
@@ -524,26 +538,26 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
 #pragma unroll
     for (int i = 0; i < NLD; ++i) {
       const int row = lrow + RSTEP * i;
-      bf16_t* dst = tile[buf] + row * HD;
+      E* dst = tile[buf] + row * HD;
       const int sw = tile_swz<HD>(row & 15);
       if constexpr (FMT == PF_BF16) {
         const uint32_t w[4] = {pf[i].x, pf[i].y, pf[i].z, pf[i].w};
         bool bad = false;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          bad |= (w[e] & 0x7f80u) == 0x7f80u || (w[e] & 0x7f800000u) == 0x7f800000u;
+          bad |= (w[e] & 0x7fffu) > Key::top || (w[e] >> 16 & 0x7fffu) > Key::top;
         // the whole row is bad where one of its lanes is
         const unsigned long long g = __ballot(bad) >> (lane & ~(TPR - 1)) & ((1ull << TPR) - 1);
         if (g) pf[i] = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(dst + 8 * (lch ^ sw)) = pf[i];
+        *reinterpret_cast<uint4*>(dst + 8 * (lch ^ sw)) = bf16_pairs<E>(pf[i]);
         if (lch == 0) poison[buf][row] = g ? __uint_as_float(0x7fc00000u) : 0.f;
         bad_any |= g != 0;
       } else {
-        const bool bad = code[i] == kScaleNan;
-        const float sc = row_scale(bad ? 127 : code[i]);
+        const bool bad = code[i] > Key::top;
+        const float sc = Key::held * row_scale(bad ? 127 : code[i]);
         const uint32_t keep = bad ? 0u : 0xffffffffu;
-        const uint2 a = dequant4_bf16<FMT>(pf[i].x & keep, sc), b = dequant4_bf16<FMT>(pf[i].y & keep, sc);
-        const uint2 c = dequant4_bf16<FMT>(pf[i].z & keep, sc), d = dequant4_bf16<FMT>(pf[i].w & keep, sc);
+        const uint2 a = dequant4<FMT, E>(pf[i].x & keep, sc), b = dequant4<FMT, E>(pf[i].y & keep, sc);
+        const uint2 c = dequant4<FMT, E>(pf[i].z & keep, sc), d = dequant4<FMT, E>(pf[i].w & keep, sc);
         *reinterpret_cast<uint4*>(dst + 8 * ((2 * lch) ^ sw)) = make_uint4(a.x, a.y, b.x, b.y);
         *reinterpret_cast<uint4*>(dst + 8 * ((2 * lch + 1) ^ sw)) = make_uint4(c.x, c.y, d.x, d.y);
         if (lch == 0) poison[buf][row] = bad ? __uint_as_float(0x7fc00000u) : 0.f;
@@ -574,7 +588,7 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
     const int tok = rr / p.nh;
     head[u] = rr - tok * p.nh;
     const T* qrow = static_cast<const T*>(p.q) + ((long long)sq.row0 * p.nh + rr) * HD;
-    w[u].template init_always<T>(qrow, live, p.normalize_q != 0, p.scale);
+    w[u].template init_always<T>(qrow, live, p.normalize_q != 0, p.scale / Key::held);
     const RowKeys k = row_keys(p, sq, sp, tok, k1);
     // (a padding row is never stored: it masks nothing)
     vis[u] = live ? k.vis : k1;
@@ -588,20 +602,20 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
   }
 
   // 32 keys (tile rows from `rows`, key index j0 of the first)
-  auto keys32 = [&](const bf16_t* rows, const float* pz, bool bad, uint32_t j0) {
+  auto keys32 = [&](const E* rows, const float* pz, bool bad, uint32_t j0) {
     f32x4 sa[QW], sb[QW];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      bf16x8 kf[W::NS];
+      v8 kf[W::NS];
 #pragma unroll
-      for (int s = 0; s < W::NS; ++s) kf[s] = *reinterpret_cast<const bf16x8*>(rows + 16 * HD * h + to.key(s));
+      for (int s = 0; s < W::NS; ++s) kf[s] = *reinterpret_cast<const v8*>(rows + 16 * HD * h + to.key(s));
 #pragma unroll
       for (int u = 0; u < QW; ++u) {
         if (h == 0) sa[u] = w[u].scores(kf);
         else sb[u] = w[u].scores(kf);
       }
     }
-    bf16x8 pb[QW];
+    v8 pb[QW];
 #pragma unroll
     for (int u = 0; u < QW; ++u) {
       float sc[8] = {sa[u][0], sa[u][1], sa[u][2], sa[u][3], sb[u][0], sb[u][1], sb[u][2], sb[u][3]};
@@ -624,10 +638,10 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int t = 0; t < W::NT; ++t) {
-      const bf16x8 va = W::vt_frag(rows, to, t);
+      const v8 va = W::vt_frag(rows, to, t);
 #pragma unroll
       for (int u = 0; u < QW; ++u)
-        w[u].o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb[u], w[u].o[t], 0, 0, 0);
+        w[u].o[t] = Mfma16<E>::run(va, pb[u], w[u].o[t]);
     }
     __builtin_amdgcn_s_setprio(0);
   };
@@ -666,7 +680,7 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
     if (u > 0) wave_lds_sync();
     if (r >= nrow) break;
     w[u].finalize();
-    store_group<HD, T>(p, w[u], (long long)sq.row0 * p.nh + r, min(16, nrow - r), whole, head[u], stage);
+    store_group<HD, FMT, T>(p, w[u], (long long)sq.row0 * p.nh + r, min(16, nrow - r), whole, head[u], stage);
   }
 }
 

@@ -185,7 +185,8 @@ def hca_paged_attention(q, rows, scales, block_table, ring_table, slots, cu_seql
     of ``ctx_lens`` (it lays the work out). Returns ``[N, nh, c]`` in ``q.dtype``, or
     writes ``out``; rows behind the last sequence, and of a longer chunk past ``max_len``,
     are zeros, in ``out`` as they were.
-    The products are bf16 with fp32 sums whatever ``q``'s type.
+    The products are bf16 with fp32 sums, for fp16 ``q`` fp16: there a row with values past
+    fp16's range reads as NaN.
     """
     fn = "hca_paged_attention"
     fmt, dev, P, page, c, n_slots, nbp, nrp, S = _step(fn, rows, scales, block_table, ring_table, slots,

@@ -692,3 +692,75 @@ def test_cache_refuses_capture(dev, monkeypatch):
                 f()
     assert cache.n_free_pages == free and cache.n_tokens(s) == n
     assert torch.equal(cache.forward_step(x[:, None]), out)
+
+
+# fp16 queries: both products in fp16, its half step u = 2^-11. Below its normal range a
+# rounding is off by at most 2^-25 instead (of a key at a quarter 2^-23, of a bf16 key, cut,
+# 2^-24): of the query sqrt(c) 2^-25 <= 2^-21 in a score of unit vectors, of the keys sqrt(c)
+# 2^-23 <= 2^-19, of each weight 2^-25 beside a sum of at least 1, and of the keys 2^-23 in the output.
+FP16 = [
+    ([1], [5003], 128, 128, 16, 128, 16, "bf16", 11.3),
+    ([1, 1, 1], [40, 4095, 16383], 4, 77, 16, 128, 64, "e4m3", 11.3),
+    ([8, 1, 3, 5], [100, 0, 63, 8190], 64, 16, 4, 64, 32, "int8", 8.0),
+    ([2, 7], [15, 16], 16, 1, 16, 128, 1, "e4m3", 1.0),
+    ([130, 1, 77], [0, 3000, 512], 16, 128, 16, 128, 32, "bf16", 11.3),
+    ([40, 170], [9000, 20000], 8, 0, 2, 64, 64, "e4m3", 5.0),
+    ([64], [700], 4, 33, 1, 128, 16, "int8", -11.3),
+]
+
+
+def fp16_tol(out, mag, scale, keys, kmax, knorm):
+    u = 2.0 ** -11
+    w = np.expm1(2 * abs(scale) * knorm * (u + 2.0 ** -18)) + u
+    return (w * mag + keys * 2.0 ** -25 * kmax + 2.0 ** -23) * (1 + u) + u * np.abs(out) + 1e-5
+
+
+@pytest.mark.parametrize("i", range(len(FP16)))
+def test_attention_fp16_products(dev, i):
+    lens, ctx, m2, win, nh, c, page, store, scale = FP16[i]
+    rng = np.random.default_rng(500 + i)
+    slots = list(rng.permutation(len(lens)))
+    pool = ref.Pool(len(lens), *pages_for(lens, ctx, m2, win, page), page, c, store, seed=i)
+    fill(pool, lens, ctx, slots, m2, win, rng)
+    q = torch.from_numpy(rng.standard_normal((sum(lens), nh, c))).to("cuda", torch.float16)
+    snk = rng.standard_normal(nh).astype(np.float32)
+    out = run_attention(pool, q, lens, ctx, slots, m2, win, snk, scale)
+    want, mag = ref.attention(pool, f64(q), lens, ctx, slots, m2=m2, win=win, sink=snk, scale=scale)
+    keys = max((x + n) // m2 for x, n in zip(ctx, lens)) + win
+    tol = fp16_tol(want, mag, scale, keys, 1.0, 1 + 2.0 ** -4)
+    assert (np.abs(f64(out) - want) <= tol).all(), np.abs(f64(out) - want).max()
+
+
+@pytest.mark.parametrize("store", ["bf16", "e4m3", "int8"])
+@pytest.mark.parametrize("n", [1, 20])
+def test_attention_fp16_rows_at_the_edge_of_its_range(dev, store, n):
+    """Rows of fp16 values up to its largest are answered, rows past it are NaN to those that see them."""
+    rng = np.random.default_rng(9)
+    m2, win, c, nh, ctx = 4, 16, 64, 4, 100
+    pool = ref.Pool(1, *pages_for([n], [ctx], m2, win, 32), 32, c, store)
+    nb = (ctx + n) // m2
+    big = 65504.0 * rng.choice([-1.0, 1.0, 0.999, 0.5, 2.0 ** -9], (nb, c))
+    pool.put(pool.blocks, 0, np.arange(nb), big)
+    pos = np.arange(ctx - win + 1, ctx + n)
+    pool.put(pool.ring, 0, pos % pool.cap, 65504.0 * rng.uniform(-1, 1, (len(pos), c)))
+    q = torch.from_numpy(rng.standard_normal((n, nh, c))).to("cuda", torch.float16)
+    scale = 2.0 ** -19
+    out = run_attention(pool, q, [n], [ctx], [0], m2, win, None, scale, normalize_q=False)
+    want, mag = ref.attention(pool, f64(q), [n], [ctx], [0], m2=m2, win=win, sink=None, scale=scale,
+                              normalize_q=False)
+    # fp16 queries are exact; a bf16 row's 65536 is taken as 65504, 2^-11 of it, which moves its
+    # score by at most |scale| 2^5 sum |q|
+    u, moved = 2.0 ** -11, scale * 2.0 ** 5 * np.abs(f64(q)).sum(-1).max()
+    tol = (np.expm1(2 * moved) + 2 * u) * mag * (1 + u) + u * np.abs(want) + (nb + win) * 2.0 ** -25 * 65536 + 1e-5
+    assert (np.abs(want) <= 65504).all()
+    assert (np.abs(f64(out) - want) <= tol).all(), np.abs(f64(out) - want).max()
+    if store == "bf16":
+        b = (ctx + n) // m2 - 1  # the last block's row, which only the last queries see
+        pool.put(pool.blocks, 0, np.array([b]), np.full((1, c), 2.0 ** 17))
+    else:
+        b = (ctx + n) // m2 - 1
+        pool.put(pool.blocks, 0, np.array([b]), np.full((1, c), 2.0 ** 19))
+    poisoned = run_attention(pool, q, [n], [ctx], [0], m2, win, None, scale, normalize_q=False)
+    sees = torch.from_numpy((ctx + np.arange(n) + 1) // m2 > b).cuda()
+    assert sees.any() and torch.isnan(poisoned[sees]).all()
+    assert torch.equal(poisoned[~sees], out[~sees])
