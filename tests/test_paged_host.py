@@ -3,8 +3,6 @@
 
 from __future__ import annotations
 
-import ctypes
-
 import numpy as np
 import pytest
 import torch
@@ -172,7 +170,6 @@ def test_references_agree_with_the_oracle():
     Cn, Zn = np.concatenate([C, C[:2]]), np.concatenate([Z, Z[:2]])
     whole = ref.append(Cn, Zn, Bp, [T + 2], [0], [0], np.zeros((1, 3, c)), m2=m2)[0]
     assert np.abs(more[0, T // m2] - whole[0, T // m2]).max() < 1e-12
-    assert ctypes.sizeof(ctypes.c_void_p) == 8
 
 
 def test_quantize_w4_of_a_transposed_weight():
