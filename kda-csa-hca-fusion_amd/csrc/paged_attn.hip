@@ -32,15 +32,19 @@
 // A key row that is not finite (E8M0 code 255, or a non-finite bf16 channel)
 // sits in LDS as zeros beside a NaN that is added to its scores: rows that do
 // not see it stay as they are (0 times NaN would reach them in the second
-// product), rows that do become NaN.
+// product), rows that do become NaN. A NaN among the e4m3 codes of a row is looked for
+// where it matters, in a step that some row masks: its scores are NaN, and then the
+// values go into the second product with zeros in its place (values_or_zero).
+// (It costs 3%; looked for in the codes themselves 5 to 10%, with a copy of the products for
+// it, which spills, 40%.)
 //
 // Measured (16 heads of 128, e4m3 rows, blocks of 128 tokens, a window of 128):
-//   one token for each of 128 contexts of 512K to 1M tokens  28.9 us + 4.9 the join, for
+//   one token for each of 128 contexts of 512K to 1M tokens  28.8 us + 4.4 the join, for
 //     99.6 MB 3.4 TB/s (a large copy 5.1): bound by the rows' bytes, and by ranges that
 //     end at different times
-//   one token behind 5003, 51 KB  9.7 us: latencies one after another (the step's
+//   one token behind 5003, 51 KB  9.6 us: latencies one after another (the step's
 //     arrays, page entries, rows, the waves' join)
-//   up to 2048 tokens behind 64K to 128K in each of 8 sequences  125 us, 565 TFLOP/s: the
+//   up to 2048 tokens behind 64K to 128K in each of 8 sequences  127 to 131 us, 550 TFLOP/s: the
 //     issue of vector instructions beside the products (71 a 16 products, most of them
 //     the softmax; products busy for 38% of the cycles)
 
@@ -113,6 +117,20 @@ __device__ __forceinline__ int computed_rows(const PagedAttnParams& p, const Pag
 // The type of the products for queries of type T.
 template <typename T> struct Prod { typedef bf16_t type; };
 template <> struct Prod<_Float16> { typedef _Float16 type; };
+
+// Whether a lane of the wave holds a NaN.
+__device__ __forceinline__ bool any_nan(const float (&sc)[8]) {
+  bool n = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) n |= sc[e] != sc[e];
+  return __ballot(n) != 0ull;
+}
+// Eight values, 0 for NaN.
+template <typename V> __device__ __forceinline__ V values_or_zero(V v) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = v[e] == v[e] ? v[e] : 0;
+  return v;
+}
 
 // One 16-row group's output, or its partial sums for the join of its ranges.
 template <int HD, int FMT, typename T, typename E>
@@ -347,6 +365,7 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
         }
       }
       v8 pb8[QW];
+      bool holes = false;  // a NaN that some row does not see
 #pragma unroll
       for (int u = 0; u < QW; ++u) {
         float sc[8] = {ra[u][0], ra[u][1], ra[u][2], ra[u][3], rb[u][0], rb[u][1], rb[u][2], rb[u][3]};
@@ -356,6 +375,7 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
         }
         const uint32_t la = blk ? 0 : lo[u], lb = blk ? vis[u] : hi[u];
         if (__ballot(j0 < la || j0 + 32 > lb)) {
+          if constexpr (FMT == PF_E4M3) holes |= any_nan(sc);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const uint32_t j = j0 + 4 * q4 + (e < 4 ? e : 12 + e);
@@ -366,7 +386,8 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
       }
 #pragma unroll
       for (int t = 0; t < W::NT; ++t) {
-        const v8 va = W::vt_frag(stage, to, t);
+        v8 va = W::vt_frag(stage, to, t);
+        if (FMT == PF_E4M3 && holes) va = values_or_zero(va);
 #pragma unroll
         for (int u = 0; u < QW; ++u)
           w[u].o[t] = Mfma16<E>::run(va, pb8[u], w[u].o[t]);
@@ -446,7 +467,8 @@ __device__ __forceinline__ RowKeys row_keys(const PagedAttnParams& p, const Page
 // to 2048 tokens behind 128K. Two groups a wave on half as many waves, with the next
 // step's scores between this one's softmax, halve the LDS reads and nearly the vector
 // instructions, but two waves a SIMD wait for LDS: 122 us there, and 76 where this
-// takes 71 for 16 chunks without a context, 167 where it takes 143 on bf16 rows.
+// takes 71 for 16 chunks without a context, 167 where it takes 143 on bf16 rows (125 us
+// for this one then).
 template <int HD, int FMT, int RG, int QW, typename T>
 __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_kernel(PagedAttnParams p) {
   typedef typename Prod<T>::type E;
@@ -616,6 +638,7 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
       }
     }
     v8 pb[QW];
+    bool holes = false;  // a NaN that some row does not see
 #pragma unroll
     for (int u = 0; u < QW; ++u) {
       float sc[8] = {sa[u][0], sa[u][1], sa[u][2], sa[u][3], sb[u][0], sb[u][1], sb[u][2], sb[u][3]};
@@ -624,6 +647,7 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
         for (int e = 0; e < 8; ++e) sc[e] += pz[4 * q4 + (e < 4 ? e : 12 + e)];
       }
       if (!(j0 + 32 <= first[u].vis || (j0 >= final_[u].lo && j0 + 32 <= first[u].hi))) {
+        if constexpr (FMT == PF_E4M3) holes |= any_nan(sc);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const uint32_t j = j0 + 4 * q4 + (e < 4 ? e : 12 + e);
@@ -638,7 +662,8 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int t = 0; t < W::NT; ++t) {
-      const v8 va = W::vt_frag(rows, to, t);
+      v8 va = W::vt_frag(rows, to, t);
+      if (FMT == PF_E4M3 && holes) va = values_or_zero(va);
 #pragma unroll
       for (int u = 0; u < QW; ++u)
         w[u].o[t] = Mfma16<E>::run(va, pb[u], w[u].o[t]);

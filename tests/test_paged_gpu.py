@@ -764,3 +764,28 @@ def test_attention_fp16_rows_at_the_edge_of_its_range(dev, store, n):
     sees = torch.from_numpy((ctx + np.arange(n) + 1) // m2 > b).cuda()
     assert sees.any() and torch.isnan(poisoned[sees]).all()
     assert torch.equal(poisoned[~sees], out[~sees])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("n", [4, 40])
+def test_attention_nan_codes_reach_only_who_sees_them(dev, dtype, n):
+    """An e4m3 NaN in one channel of a row: NaN for the queries that see it, nothing for the others."""
+    rng = np.random.default_rng(11)
+    m2, win, c, nh, ctx = 4, 8, 64, 4, 61
+    pool = ref.Pool(1, *pages_for([n], [ctx], m2, win, 32), 32, c, "e4m3")
+    fill(pool, [n], [ctx], [0], m2, win, rng)
+    q = torch.from_numpy(rng.standard_normal((n, nh, c))).to("cuda", DT[dtype])
+    clean = run_attention(pool, q, [n], [ctx], [0], m2, win, None, 8.0)
+    b = (ctx + n) // m2 - 1
+    pos = ctx + np.arange(n)
+    raw = pool.rows.view(torch.uint8)
+    for table, at, sees in ((pool.blocks, b, (pos + 1) // m2 > b),
+                            (pool.ring, (ctx + 2) % pool.cap, (pos >= ctx + 2) & (pos < ctx + 2 + win))):
+        page, line = int(table[0, at // 32]), at % 32
+        held = int(raw[page, line, c - 3])
+        raw[page, line, c - 3] = 0xff
+        out = run_attention(pool, q, [n], [ctx], [0], m2, win, None, 8.0)
+        raw[page, line, c - 3] = held
+        sees = torch.from_numpy(sees).cuda()
+        assert sees.any() and (~sees).any()
+        assert torch.isnan(out[sees]).all() and torch.equal(out[~sees], clean[~sees])
