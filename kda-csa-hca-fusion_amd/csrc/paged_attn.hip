@@ -385,12 +385,18 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
         pb8[u] = w[u].softmax32(sc);
       }
 #pragma unroll
-      for (int t = 0; t < W::NT; ++t) {
-        v8 va = W::vt_frag(stage, to, t);
-        if (FMT == PF_E4M3 && holes) va = values_or_zero(va);
+      for (int t0 = 0; t0 < W::NT; t0 += 4) {
+        v8 va[4];
 #pragma unroll
-        for (int u = 0; u < QW; ++u)
-          w[u].o[t] = Mfma16<E>::run(va, pb8[u], w[u].o[t]);
+        for (int t = 0; t < 4; ++t) va[t] = W::vt_frag(stage, to, t0 + t);
+        if (FMT == PF_E4M3 && holes) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) va[t] = values_or_zero(va[t]);
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int u = 0; u < QW; ++u) w[u].o[t0 + t] = Mfma16<E>::run(va[t], pb8[u], w[u].o[t0 + t]);
       }
     };
 
@@ -623,6 +629,10 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
     final_[u] = row_keys(p, sq, sp, g1 / p.nh, k1);
   }
 
+  // values read this many 16-column tiles ahead of their products: four, where 128 registers
+  // hold them beside the e4m3 rows' look for NaN (that spills at 128 columns: 156 us for 116; bf16
+  // rows 138 for 142, 64 columns 78 for 81)
+  constexpr int kPv = RG == 8 && HD == 128 && FMT == PF_E4M3 ? 1 : 4;
   // 32 keys (tile rows from `rows`, key index j0 of the first)
   auto keys32 = [&](const E* rows, const float* pz, bool bad, uint32_t j0) {
     f32x4 sa[QW], sb[QW];
@@ -661,12 +671,18 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
     // 82.6 -> 76.8 us, long ones 126 -> 122)
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int t = 0; t < W::NT; ++t) {
-      v8 va = W::vt_frag(rows, to, t);
-      if (FMT == PF_E4M3 && holes) va = values_or_zero(va);
+    for (int t0 = 0; t0 < W::NT; t0 += kPv) {
+      v8 va[kPv];
 #pragma unroll
-      for (int u = 0; u < QW; ++u)
-        w[u].o[t] = Mfma16<E>::run(va, pb[u], w[u].o[t]);
+      for (int t = 0; t < kPv; ++t) va[t] = W::vt_frag(rows, to, t0 + t);
+      if (FMT == PF_E4M3 && holes) {
+#pragma unroll
+        for (int t = 0; t < kPv; ++t) va[t] = values_or_zero(va[t]);
+      }
+#pragma unroll
+      for (int t = 0; t < kPv; ++t)
+#pragma unroll
+        for (int u = 0; u < QW; ++u) w[u].o[t0 + t] = Mfma16<E>::run(va[t], pb[u], w[u].o[t0 + t]);
     }
     __builtin_amdgcn_s_setprio(0);
   };
