@@ -232,25 +232,13 @@ def run(s):
             "w4": _plain_w4}[kind](s)
 
 
-_kch = None
-
-
-def _package():
-    """The framework, imported once."""
-    global _kch
+def _own(s):
     import os
     import sys
     pkg = os.path.abspath("kda-csa-hca-fusion_amd")
     if pkg not in sys.path:
         sys.path.insert(0, pkg)
     import kch
-    _kch = kch
-
-
-def _own(s):
-    if _kch is None:
-        _package()
-    kch = _kch
     kind = s["kind"]
     if kind == "w4":
         return kch.linear_w4(s["x"], s["packed"], s["scales"], s["zeros"], residual=s["residual"])
