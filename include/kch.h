@@ -574,7 +574,7 @@ int kch_linear_up(const void* x, long long ldx, const void* w, long long ldw, vo
  * (rows outside 0 .. N - 1, a slot outside the tables, a negative position)
  * are passed over. A table entry that names no page of the pool reads as a row of
  * zeros and is not written. max_len is at least the longest chunk (the attention
- * leaves a longer one's rows past it as they were, or zeros with zero_tail).
+ * does not answer a longer one's rows past it).
  */
 
 /*
@@ -607,8 +607,9 @@ int kch_hca_paged_append(const void* C, long long ldc, const void* Z, long long 
  * ctx (it lays the work out; a larger one is answered rightly, if slower).
  * The products take bf16, with dtype fp16 fp16: rows with values past its range
  * then read as NaN (kept in 8 bits, past four times its range).
- * Rows of out that belong to no sequence behind cu[S] are left as they were, or
- * zeros with zero_tail. ws as kch_hca_paged_attn_ws_bytes says, 256-byte aligned.
+ * Rows of out that no sequence answers (ahead of cu[0], behind cu[S], of a sequence
+ * that is passed over, of a chunk past max_len) are left as they were, or zeros with
+ * zero_tail. ws as kch_hca_paged_attn_ws_bytes says, 256-byte aligned.
  */
 size_t kch_hca_paged_attn_ws_bytes(int S, int N, int nh, int c, int m2, int win, int max_len, int max_ctx);
 int kch_hca_paged_attn(const void* q, const float* sink, void* out, const void* rows, const void* scales,
@@ -621,7 +622,7 @@ int kch_hca_paged_attn(const void* q, const float* sink, void* out, const void* 
 /*
  * Cached rows back as numbers: output row cu[i] + j is row (first[i] + j) %
  * (nbp page) of slot slots[i]'s pages in table [n_slots, nbp] (either table
- * above; first NULL: 0). out [N, c] of odtype; rows behind cu[S] as above.
+ * above; first NULL: 0). out [N, c] of odtype; rows ahead of cu[0] and behind cu[S] as above.
  */
 int kch_paged_read(const void* rows, const void* scales, const int* table, const int* slots, const int* cu,
                    const int* first, void* out, int S, int N, int c, int P, int page, int nbp, int n_slots,

@@ -454,7 +454,7 @@ hipError_t paged_append_dispatch(const PagedAppendParams& p, int format, int dty
 struct PagedReadParams {
   PagedPool pool;         // block_table: the table that is read; ctx: first row or null; N output rows
   void* out;              // [N, c]
-  int zero_tail;          // rows behind the last sequence are written as zeros
+  int zero_tail;          // rows of no sequence are written as zeros
 };
 hipError_t paged_read_dispatch(const PagedReadParams& p, int format, int odtype, hipStream_t s);
 struct PagedAttnParams {

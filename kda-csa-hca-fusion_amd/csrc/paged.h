@@ -117,22 +117,22 @@ template <typename E> __device__ __forceinline__ uint4 bf16_pairs(uint4 v) {
   return make_uint4(bf16_pair<E>(v.x), bf16_pair<E>(v.y), bf16_pair<E>(v.z), bf16_pair<E>(v.w));
 }
 
-// A sequence of the step: its slot, first row and length (0 where the arrays do
-// not describe rows of this call), and the tokens cached before it. Positions
-// are below 2^32: ctx and len are ints.
+// A sequence of the step: its slot, the rows that the arrays give it, its length (0
+// where they do not describe rows of this call: it is passed over), and the tokens
+// cached before it. Positions are below 2^32: ctx and len are ints.
 struct PagedSeq {
-  int slot, row0, len;
+  int slot, row0, end, len;
   uint32_t ctx;
 };
 __device__ __forceinline__ PagedSeq paged_seq(const PagedPool& p, int i) {
   PagedSeq s;
   s.slot = p.slots[i];
   s.row0 = p.cu[i];
-  const int end = p.cu[i + 1];
+  s.end = p.cu[i + 1];
   const int ctx = p.ctx[i];
   s.ctx = (uint32_t)ctx;
-  s.len = end - s.row0;
-  if (s.row0 < 0 || end > p.N || end < s.row0 || s.slot < 0 || s.slot >= p.n_slots || ctx < 0) s.len = 0;
+  s.len = s.end - s.row0;
+  if (s.row0 < 0 || s.end > p.N || s.end < s.row0 || s.slot < 0 || s.slot >= p.n_slots || ctx < 0) s.len = 0;
   return s;
 }
 

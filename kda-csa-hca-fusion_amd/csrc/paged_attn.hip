@@ -101,14 +101,30 @@ __device__ __forceinline__ void zero_rows(const PagedAttnParams& p, long long n0
   for (long long i = n0 * HD + 4ll * threadIdx.x; i < n1 * HD; i += 4ll * blockDim.x)
     Store4<T>::run(static_cast<T*>(p.out) + i, f32x4{0.f, 0.f, 0.f, 0.f}, 1.f);
 }
-// The rows that no workgroup computes: those behind the last sequence (a share of each
-// workgroup of a grid row of their own), and what a chunk has past max_len.
+// Rows [r0, r1) as zeros, a share of each workgroup of the grid row.
 template <int HD, typename T>
-__device__ __forceinline__ void zero_tail(const PagedAttnParams& p) {
-  if (blockIdx.z) return;
-  const long long r0 = (long long)max(0, min(p.pool.cu[p.pool.S], p.pool.N)) * p.nh, r1 = (long long)p.pool.N * p.nh;
+__device__ __forceinline__ void zero_shared(const PagedAttnParams& p, long long r0, long long r1) {
   const long long per = (r1 - r0 + gridDim.x - 1) / gridDim.x, at = r0 + per * blockIdx.x;
   zero_rows<HD, T>(p, at, min(r1, at + per));
+}
+// The rows that no workgroup computes, as zeros: those ahead of the first and behind the last
+// sequence (a grid row of their own), the whole chunk of a sequence that is passed over,
+// and what a chunk has past max_len.
+template <int HD, typename T>
+__device__ __forceinline__ void zero_ends(const PagedAttnParams& p) {
+  if (blockIdx.z) return;
+  const long long nh = p.nh, N = p.pool.N;
+  zero_shared<HD, T>(p, 0, nh * max(0, min(p.pool.cu[0], p.pool.N)));
+  zero_shared<HD, T>(p, nh * max(0, min(p.pool.cu[p.pool.S], p.pool.N)), nh * N);
+}
+template <int HD, typename T>
+__device__ __forceinline__ void zero_rest(const PagedAttnParams& p, const PagedSeq& sq) {
+  if (!p.zero_tail || blockIdx.z) return;
+  const long long nh = p.nh;
+  if (sq.len == 0)
+    zero_shared<HD, T>(p, nh * max(0, min(sq.row0, p.pool.N)), nh * min(sq.end, p.pool.N));
+  else if (sq.len > p.max_len)
+    zero_shared<HD, T>(p, nh * (sq.row0 + p.max_len), nh * (sq.row0 + sq.len));
 }
 __device__ __forceinline__ int computed_rows(const PagedAttnParams& p, const PagedSeq& sq) {
   return min(sq.len, p.max_len) * p.nh;  // N nh is below 2^30
@@ -174,11 +190,10 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
   __shared__ float ml[4][16][2];
   __shared__ float poison[4][32];
   const PagedPool& pl = p.pool;
-  if (blockIdx.y == (unsigned)pl.S) return zero_tail<HD, T>(p);
+  if (blockIdx.y == (unsigned)pl.S) return zero_ends<HD, T>(p);
   const PagedSeq sq = paged_seq(pl, blockIdx.y);
   const int nrow = computed_rows(p, sq);
-  if (p.zero_tail && sq.len > p.max_len && !(blockIdx.x | blockIdx.z))
-    zero_rows<HD, T>(p, (long long)sq.row0 * p.nh + nrow, (long long)(sq.row0 + sq.len) * p.nh);
+  zero_rest<HD, T>(p, sq);
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int lane = lane_id(), q4 = lane >> 4, n = lane & 15;
   const int lrow = lane / TPR, lch = lane % TPR;
@@ -494,11 +509,10 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
 
   const int tid = threadIdx.x;
   const PagedPool& pl = p.pool;
-  if (blockIdx.y == (unsigned)pl.S) return zero_tail<HD, T>(p);
+  if (blockIdx.y == (unsigned)pl.S) return zero_ends<HD, T>(p);
   const PagedSeq sq = paged_seq(pl, blockIdx.y);
   const int nrow = computed_rows(p, sq);
-  if (p.zero_tail && sq.len > p.max_len && !(blockIdx.x | blockIdx.z))
-    zero_rows<HD, T>(p, (long long)sq.row0 * p.nh + nrow, (long long)(sq.row0 + sq.len) * p.nh);
+  zero_rest<HD, T>(p, sq);
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, q4 = lane >> 4, n = lane & 15;
   const uint32_t ring_cap = (uint32_t)pl.nrp << pl.log2page;

@@ -183,8 +183,10 @@ def hca_paged_attention(q, rows, scales, block_table, ring_table, slots, cu_seql
     ``max(0, p - sliding_window + 1) .. p`` in one softmax with the sink; 0 where it
     sees none. ``max_len`` is at least the longest chunk, ``max_ctx`` at least the largest
     of ``ctx_lens`` (it lays the work out). Returns ``[N, nh, c]`` in ``q.dtype``, or
-    writes ``out``; rows behind the last sequence, and of a longer chunk past ``max_len``,
-    are zeros, in ``out`` as they were.
+    writes ``out``. Rows that no sequence answers are zeros, in ``out`` as they were: ahead of
+    the first sequence and behind the last, of a longer chunk past ``max_len``, and of a
+    sequence that is passed over (a slot outside the table, as a padding entry has it, a negative
+    context, rows outside ``q``).
     The products are bf16 with fp32 sums, for fp16 ``q`` fp16: there a row with values past
     fp16's range reads as NaN.
     """
@@ -236,7 +238,7 @@ def paged_read(rows, scales, table, slots, cu_rows, *, total, first=None, dtype=
     """Rows of a paged cache as numbers, packed: row ``cu_rows[i] + j`` of the result is
     row ``(first[i] + j) % capacity`` of slot ``slots[i]`` in ``table`` (a block or a ring
     table), capacity its pages times their rows. ``total`` is the number of result rows; those
-    behind the last sequence are zeros (in ``out`` as they were)."""
+    ahead of the first sequence and behind the last are zeros (in ``out`` as they were)."""
     fn = "paged_read"
     fmt, dev, P, page, c, n_slots, nbp, _, S = _step(fn, rows, scales, table, None, slots, cu_rows, first)
     if total < 0:

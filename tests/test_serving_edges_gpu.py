@@ -1,0 +1,61 @@
+"""Edges of the serving operators on the GPU: steps that say nothing or too much, masks of the type's
+lowest value, rows that are not finite, and how many bits the products keep."""
+
+from __future__ import annotations
+
+import numpy as np
+import paged_ref as ref
+import pytest
+import torch
+from test_paged_gpu import DT, f64, fill, pages_for, run_attention
+
+pytestmark = pytest.mark.gpu
+
+
+# --------------------------------------------------------------------------- rows that nothing answers
+
+@pytest.mark.parametrize("nh,lens,max_len", [
+    (4, [3, 2, 4, 1], 4), (16, [2, 1, 2, 1], 2), (16, [3, 40, 30, 5], 40), (4, [3, 40, 90, 5], 20), (16, [1, 1, 9, 1], 1),
+])
+def test_rows_of_sequences_passed_over_are_zeros(dev, nh, lens, max_len, monkeypatch):
+    """A fresh result holds zeros, never what its memory held before: rows ahead of the first sequence, of slots
+    outside the table, of a negative context and behind the last sequence. A given one keeps them."""
+    import kch
+    rng = np.random.default_rng(31)
+    m2, win, c = 16, 16, 64
+    ctx = [100, 90, 80, 70]
+    pool = ref.Pool(4, *pages_for(lens, ctx, m2, win, 16), 16, c, "e4m3")
+    fill(pool, lens, ctx, [0, 1, 2, 3], m2, win, rng)
+    n = sum(lens)
+    q = torch.from_numpy(rng.standard_normal((2 + n + 5, nh, c))).cuda().bfloat16()
+    s, cu, cx, _ = ref.step(lens, ctx, [0, 1, 2, 3])
+
+    def go(out=None):
+        return kch.hca_paged_attention(q, pool.rows, pool.scales, pool.blocks, pool.ring, s, cu + 2, cx, m2=m2,
+                                       sliding_window=win, max_len=max_len, max_ctx=200, scale=8.0, out=out)
+
+    whole = go().clone()
+    monkeypatch.setattr(torch, "empty_like", lambda t: torch.full_like(t, float("nan")))
+    first = go()
+    assert (first[:2] == 0).all() and (first[2 + n:] == 0).all() and torch.equal(first[2:2 + n], whole[2:2 + n])
+    at = 2 + np.concatenate([[0], np.cumsum(lens)])
+    for bad, how in ((1, "slot"), (2, "slots"), (3, "ctx"), (0, "ctx")):
+        keep = s.clone(), cx.clone()
+        if how == "ctx":
+            cx[bad] = -5
+        else:
+            s[bad] = -1 if how == "slot" else 4
+        out, mine = go(), go(torch.full_like(q, 9.0))
+        s.copy_(keep[0]), cx.copy_(keep[1])
+        for i in range(4):
+            a, b = at[i], at[i + 1]
+            if i == bad:
+                assert (out[a:b] == 0).all() and (mine[a:b] == 9.0).all()
+            else:
+                assert torch.equal(out[a:b], whole[a:b])
+        assert (out[:2] == 0).all() and (out[2 + n:] == 0).all()
+        assert (mine[:2] == 9.0).all() and (mine[2 + n:] == 9.0).all()
+    # the last sequence says it has more rows than there are
+    cu[4] = 1000
+    out = go()
+    assert (out[at[3]:] == 0).all() and torch.equal(out[2:at[3]], whole[2:at[3]])
