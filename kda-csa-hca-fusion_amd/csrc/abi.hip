@@ -1634,11 +1634,10 @@ int kch_hca_paged_attn(const void* q, const float* sink, void* out, const void* 
   if (N == 0 || ((S == 0 || max_len == 0) && !zero_tail)) return KCH_OK;
   if (!q || !out || (S > 0 && (!slots || !cu || !ctx))) return fail(KCH_ERR_INVALID, "%s: null pointer", fn);
   if (((uintptr_t)q | (uintptr_t)out) & 15) return fail(KCH_ERR_INVALID, "%s: q and out must be 16-byte aligned", fn);
-  if (S == 0)  // no sequence: every row is behind the last one
+  if (S == 0 || max_len == 0)  // no sequence, or no token of any chunk: no row is answered
     return hip_status(fn, kch::fill_u32(out, (long long)N * nh * c / (dtype == KCH_DT_F32 ? 1 : 2), 0u,
                                         (hipStream_t)stream));
   if (max_len > N) max_len = N;
-  if (max_len < 1) max_len = 1;
   const kch::PagedAttnPlan pl = kch::paged_attn_plan(S, N, nh, c, m2, win, max_len, max_ctx);
   if (pl.bytes) {
     if (!ws || ws_bytes < pl.bytes) return fail(KCH_ERR_INVALID, "%s: workspace of %zu bytes required", fn, pl.bytes);

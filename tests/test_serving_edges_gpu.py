@@ -59,3 +59,20 @@ def test_rows_of_sequences_passed_over_are_zeros(dev, nh, lens, max_len, monkeyp
     cu[4] = 1000
     out = go()
     assert (out[at[3]:] == 0).all() and torch.equal(out[2:at[3]], whole[2:at[3]])
+
+
+@pytest.mark.parametrize("lens", [[0, 0], [3, 2]])
+def test_no_token_of_any_chunk(dev, lens):
+    """max_len = 0: no row is answered, whatever the contexts' bound."""
+    import kch
+    rng = np.random.default_rng(32)
+    pool = ref.Pool(2, 1, 1, 16, 128, "int8")
+    fill(pool, [3, 2], [50, 60], [0, 1], 16, 8, rng)
+    q = torch.from_numpy(rng.standard_normal((7, 16, 128))).cuda().bfloat16()
+    s, cu, cx, _ = ref.step(lens, [50, 60], [0, 1])
+    for max_ctx in (60, 10 ** 6, None):
+        args = (pool.rows, pool.scales, pool.blocks, pool.ring, s, cu, cx)
+        kw = dict(m2=16, sliding_window=8, max_len=0, max_ctx=max_ctx)
+        assert (kch.hca_paged_attention(q, *args, **kw) == 0).all()
+        mine = torch.full_like(q, 3.0)
+        assert kch.hca_paged_attention(q, *args, out=mine, **kw) is mine and (mine == 3.0).all()
