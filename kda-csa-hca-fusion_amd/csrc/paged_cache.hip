@@ -24,6 +24,8 @@
 // 2.5 us at the rate of a large copy). Bound by what one workgroup does in a row: the
 // step's arrays, the block's rows, its sums over the waves, the quantised row.
 
+#include <cfloat>
+
 #include "paged.h"
 
 namespace kch {
@@ -52,8 +54,9 @@ template <int W> __device__ __forceinline__ float group_amax(float v) {
 }
 
 // e^(a - b) of softmax references: a = -inf (nothing summed yet) gives 0, also
-// where b is -inf.
-__device__ __forceinline__ float ref_exp(float a, float b) { return exp_hw(a - fmaxf(b, -3e38f)); }
+// where b is -inf. (A reference of the type's lowest value is one like any other: a block
+// masked with it weighs its tokens alike.)
+__device__ __forceinline__ float ref_exp(float a, float b) { return exp_hw(a - fmaxf(b, -FLT_MAX)); }
 
 // One softmax state (max, sum, weighted sum) joined into another.
 struct Sums {

@@ -76,3 +76,37 @@ def test_no_token_of_any_chunk(dev, lens):
         assert (kch.hca_paged_attention(q, *args, **kw) == 0).all()
         mine = torch.full_like(q, 3.0)
         assert kch.hca_paged_attention(q, *args, out=mine, **kw) is mine and (mine == 3.0).all()
+
+
+# --------------------------------------------------------------------------- masks and rows that are not finite
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("store", ["bf16", "e4m3", "int8"])
+def test_blocks_masked_with_the_lowest_value(dev, dtype, store):
+    """Gates of the type's lowest value: alone in a block they weigh alike (its plain mean), beside others nothing,
+    and they outweigh -inf; the sums that a chunk leaves and the next one takes up as well."""
+    import kch
+    rng = np.random.default_rng(33)
+    c, m2 = 64, 8
+    low = torch.finfo(DT[dtype]).min
+    pool = ref.Pool(1, 1, 4, 16, c, store)
+    C = torch.from_numpy(rng.standard_normal((40, c))).to("cuda", DT[dtype])
+    Z = torch.from_numpy(rng.standard_normal((40, c))).to("cuda", DT[dtype])
+    Z[0:8] = low                     # a whole block
+    Z[8:11] = low                    # some of one
+    Z[16:24], Z[18] = float("-inf"), low   # one weight left
+    Z[24:40, ::2] = low              # every other channel of two blocks
+    Bp = torch.zeros(m2, c).cuda()
+    for cut in (40, 5, 27, 16):      # ends of the first chunk
+        pool.state.fill_(7.0)
+        for a, b in ((0, cut), (cut, 40)):
+            if a == b:
+                continue
+            s, cu, cx, _ = ref.step([b - a], [a], [0])
+            kch.hca_paged_append(C[a:b], Z[a:b], Bp, pool.rows, pool.scales, pool.state, pool.blocks, pool.ring, s, cu,
+                                 cx, m2=m2, max_len=b - a)
+        rows, _, _ = ref.append(f64(C), f64(Z), f64(Bp), [40], [0], [0], np.zeros((1, 3, c)), m2=m2)
+        want = np.stack([rows[0, b] for b in range(5)])
+        got, sc = pool.get(pool.blocks, 0, np.arange(5)), pool.get_scale(pool.blocks, 0, np.arange(5))
+        tol = ref.half_step(want, sc, store) * (1 + 1e-4) + 1e-5 * np.abs(want).max(-1, keepdims=True)
+        assert (np.abs(got - want) <= tol).all(), (cut, np.abs(got - want).max())
