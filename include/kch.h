@@ -584,6 +584,7 @@ int kch_linear_up(const void* x, long long ldx, const void* w, long long ldw, vo
  * (normalize = 1) and quantised as they are written:
  *   8-bit row x, amax = max |x|: scale 2^e, e the least integer with amax <=
  *   448 2^e (e4m3) or 127 2^e (int8), 0 below 2^-100; code = rne(x / 2^e)
+ * A row with a channel that is infinite or NaN is NaN in every channel, in each format.
  * C, Z [N, c] of dtype, rows ldc / ldz elements apart (16-byte aligned), B_pos
  * [m2, c] fp32. state [n_slots, 3, c] fp32 holds, for the block that a slot's
  * last token left open, the running max, sum and weighted sum of its softmax;

@@ -6,8 +6,8 @@
 // two because then nothing past the code's own rounding is lost: e4m3 steps are
 // relative, and every value (at most 7 significant bits) is exact in bf16, so
 // the attention's products see the stored values themselves and no scale enters
-// its scores. A row with a non-finite channel has the code 255 (NaN in E8M0) and
-// reads as NaN.
+// its scores. A row that is written with a non-finite channel is NaN in every channel
+// (its norm is no number): code 255 (NaN in E8M0), or bf16 NaNs.
 #pragma once
 
 #include "attn_common.h"
@@ -34,11 +34,14 @@ template <> struct PagedFmt<PF_INT8> {
   static constexpr uint32_t top_frac = 0x7e0000u;
 };
 
+// Whether a row of this largest magnitude has a channel that is infinite or NaN.
+__device__ __forceinline__ bool not_finite(float amax) { return __float_as_uint(amax) >= 0x7f800000u; }
+
 // The E8M0 code of a row whose largest magnitude is amax (NaN or infinite: 255).
 template <int FMT>
 __device__ __forceinline__ int row_scale_code(float amax) {
   const uint32_t u = __float_as_uint(amax);
-  if (u >= 0x7f800000u) return kScaleNan;
+  if (not_finite(amax)) return kScaleNan;
   if (amax < kRowTiny) return 127;
   return (int)(u >> 23) - PagedFmt<FMT>::top_exp + ((u & 0x7fffffu) > PagedFmt<FMT>::top_frac ? 1 : 0);
 }

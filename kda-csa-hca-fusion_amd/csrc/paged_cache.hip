@@ -148,6 +148,9 @@ __global__ __launch_bounds__(64 * NWV) void paged_append_kernel(PagedAppendParam
           mx = amax_nan(mx, x[i]);
         }
         if constexpr (FMT == PF_BF16) {
+          if (not_finite(group_amax<LPR>(mx)))
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(0x7fc00000u);
           if (at[u] >= 0) *reinterpret_cast<bf16x8*>(rows + at[u] * HD + ch) = to_bf16x8(x);
         } else {
           const int code = row_scale_code<FMT>(group_amax<LPR>(mx));
@@ -221,15 +224,13 @@ __global__ __launch_bounds__(64 * NWV) void paged_append_kernel(PagedAppendParam
           x[k] *= inv;
           mx = amax_nan(mx, x[k]);
         }
-        if constexpr (FMT != PF_BF16) {
 #pragma unroll
-          for (int k = 32; k >= 1; k >>= 1) mx = amax_nan(mx, __shfl_xor(mx, k));
-        }
+        for (int k = 32; k >= 1; k >>= 1) mx = amax_nan(mx, __shfl_xor(mx, k));
         if (pr >= 0) {
           elem* dst = rows + pr * HD + CPL * lane;
           if constexpr (FMT == PF_BF16) {
 #pragma unroll
-            for (int k = 0; k < CPL; ++k) dst[k] = (bf16_t)x[k];
+            for (int k = 0; k < CPL; ++k) dst[k] = (bf16_t)(not_finite(mx) ? __uint_as_float(0x7fc00000u) : x[k]);
           } else {
             const int code = row_scale_code<FMT>(mx);
             const uint32_t w = quant4<FMT>(x[0], CPL > 1 ? x[CPL - 1] : 0.f, 0.f, 0.f, code);

@@ -110,3 +110,31 @@ def test_blocks_masked_with_the_lowest_value(dev, dtype, store):
         got, sc = pool.get(pool.blocks, 0, np.arange(5)), pool.get_scale(pool.blocks, 0, np.arange(5))
         tol = ref.half_step(want, sc, store) * (1 + 1e-4) + 1e-5 * np.abs(want).max(-1, keepdims=True)
         assert (np.abs(got - want) <= tol).all(), (cut, np.abs(got - want).max())
+
+
+@pytest.mark.parametrize("store", ["bf16", "e4m3", "int8"])
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_rows_with_a_channel_that_is_not_finite(dev, store, normalize, bad):
+    """They read as NaN in every channel, in each format, the rows beside them as they are."""
+    import kch
+    rng = np.random.default_rng(34)
+    for c, n in ((64, 24), (128, 24), (128, 1)):
+        m2 = 8
+        pool = ref.Pool(1, 1, 2, 16, c, store)
+        C = torch.from_numpy(rng.standard_normal((24, c))).float().cuda()
+        Z = torch.zeros_like(C)
+        C[20, 7], C[5, c - 1] = bad, bad
+        Bp = torch.zeros(m2, c).cuda()
+        for a in range(0, 24, n):
+            s, cu, cx, _ = ref.step([n], [a], [0])
+            kch.hca_paged_append(C[a:a + n], Z[a:a + n], Bp, pool.rows, pool.scales, pool.state, pool.blocks, pool.ring,
+                                 s, cu, cx, m2=m2, max_len=n, normalize=normalize)
+        s, cu, _, _ = ref.step([3], [0], [0])
+        keys = kch.paged_read(pool.rows, pool.scales, pool.blocks, s, cu, total=3, dtype=torch.float32)
+        s, cu, _, _ = ref.step([24], [0], [0])
+        win = kch.paged_read(pool.rows, pool.scales, pool.ring, s, cu, total=24, dtype=torch.float32)
+        assert torch.isnan(keys[[0, 2]]).all() and torch.isfinite(keys[1]).all() and keys[1].abs().max() > 0
+        ok = torch.ones(24, dtype=torch.bool)
+        ok[20] = ok[5] = False
+        assert torch.isnan(win[~ok]).all() and torch.isfinite(win[ok]).all() and (win[ok].abs().amax(-1) > 0).all()
