@@ -638,7 +638,8 @@ int kch_paged_read(const void* rows, const void* scales, const int* table, const
  * scales [K / group, N] of dtype (1 bf16, 2 fp16); zeros [K / group, N] uint8 or NULL
  * (8). group 32, 64 or 128, K a multiple of it. x, res, y of dtype with row
  * strides ldx (a multiple of 8, x 16-byte aligned), ldr, ldy. Any M >= 0; made for
- * up to 16 rows (each further 16 read the weights again).
+ * up to 16 rows (each further 16 read the weights again). Outputs whose sums are not
+ * finite are summed again term by term (slower, infinities as the formula has them).
  */
 int kch_linear_w4(const void* x, long long ldx, const void* codes, const void* scales, const void* zeros,
                   const void* res, long long ldr, void* y, long long ldy, int M, int N, int K, int group,

@@ -57,6 +57,27 @@ __device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
   w[0] = c[0]; w[1] = c[1]; w[2] = d[0]; w[3] = d[1];
 }
 
+// y[m, n] term by term, in fp64: for sums that came out infinite or NaN. An infinite x, or sums
+// of 128 x past fp32's range, meet their own negative in the offset's sum, where the
+// definition's product is an infinity or finite.
+template <typename T>
+__device__ __forceinline__ float w4_terms(const LinearW4Params& p, int m, int n) {
+  const T* const x = static_cast<const T*>(p.x) + (size_t)m * p.ldx;
+  const uint32_t* const w = reinterpret_cast<const uint32_t*>(p.w + (size_t)n * (p.K / 2));
+  double sum = 0.0;
+#pragma unroll 1
+  for (int k = 0; k < p.K; k += 8) {
+    const size_t g = (size_t)(k / p.group) * p.N + n;
+    const float s = to_f32(static_cast<const T*>(p.scales)[g]);
+    const int z = p.zeros ? p.zeros[g] : 8;
+    const uint32_t c = w[k / 8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      sum += (double)to_f32(x[k + i]) * ((double)s * ((int)(c >> (4 * i) & 15u) - z));
+  }
+  return (float)sum;
+}
+
 // What a wave holds of 128 consecutive k: its tiles' codes, x, and per group the scales
 // (4 of 16 bits) and zero points (4 bytes) of the lane's rows of y^T.
 template <int NT, int G> struct W4Piece {
@@ -236,6 +257,7 @@ __global__ __launch_bounds__(64 * KW) void linear_w4_kernel(LinearW4Params p) {
     float v = 0.f;
 #pragma unroll
     for (int w = 0; w < KW; ++w) v += part[w][m][n];
+    if (!(fabsf(v) < INFINITY)) v = w4_terms<T>(p, m0 + m, n0 + n);
     if (p.res) v += to_f32(static_cast<const T*>(p.res)[(size_t)(m0 + m) * p.ldr + n0 + n]);
     static_cast<T*>(p.y)[(size_t)(m0 + m) * p.ldy + n0 + n] = from_f32<T>(v);
   }

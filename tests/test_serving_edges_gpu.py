@@ -138,3 +138,51 @@ def test_rows_with_a_channel_that_is_not_finite(dev, store, normalize, bad):
         ok = torch.ones(24, dtype=torch.bool)
         ok[20] = ok[5] = False
         assert torch.isnan(win[~ok]).all() and torch.isfinite(win[ok]).all() and (win[ok].abs().amax(-1) > 0).all()
+
+
+# --------------------------------------------------------------------------- 4-bit weights
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("M,N,K,G,zeros", [
+    (1, 64, 256, 64, False), (5, 100, 96, 32, True), (16, 250, 512, 128, True), (3, 8212, 160, 32, True),
+    (16, 16404, 192, 64, False), (33, 40, 128, 128, True),
+])
+def test_linear_w4_of_rows_that_are_not_finite(dev, dtype, M, N, K, G, zeros):
+    """An infinite x gives the infinity of its weight's sign (NaN where the weight is zero or two of them differ), NaN
+    gives NaN, values whose sums pass fp32 on the way what their weights make of them; other rows nothing."""
+    import kch
+    from test_w4_gpu import make, weights
+    packed, scales, zp = make(N, K, G, zeros, dtype, M)
+    g = torch.Generator(device="cuda").manual_seed(K)
+    x = torch.randn(M, K, device="cuda", generator=g).to(DT[dtype])
+    res = torch.randn(M, N, device="cuda", generator=g).to(DT[dtype])
+    clean = kch.linear_w4(x, packed, scales, zp, residual=res)
+    W = weights(packed, scales, zp, G)
+    inf = float("inf")
+    rows = [{0: inf}, {K - 1: -inf}, {3: inf, K // 2: inf}, {7: float("nan")}]
+    if dtype == "bf16":
+        rows += [{1: 3e38, 2: -3e38}, {K - 2: 1.5e37, 40: -2e37}]
+    for at in rows:
+        m = M - 1
+        y = x.clone()
+        for k, v in at.items():
+            y[m, k] = v
+        out = kch.linear_w4(y, packed, scales, zp, residual=res)
+        assert torch.equal(out[:m], clean[:m]) if m else True
+        with np.errstate(invalid="ignore", over="ignore"):
+            xs = f64(y[m])
+            want = np.array([sum(xs[k] * W[:, k] for k in at)]) + f64(res[m])
+            rest = xs.copy()
+            rest[list(at)] = 0.0
+            want = torch.from_numpy(want[0] + W @ rest).to(DT[dtype]).float()
+        got = out[m].float().cpu()
+        assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got), torch.isinf(want))
+        assert (torch.sign(got) == torch.sign(want))[torch.isinf(want)].all()
+        ok = torch.isfinite(want)
+        # two roundings (this reference's and the operator's): a step apart at most. Where two terms past fp32's
+        # sums cancel (equal weights), what was added between them is gone: a 64-bit sum of K terms is off by up to
+        # K 2^-53 of the sum of their magnitudes, in whatever order
+        with np.errstate(invalid="ignore", over="ignore"):
+            lost = torch.from_numpy(K * 2.0 ** -53 * (np.abs(W) @ np.abs(xs)))
+        tol = 2 * torch.finfo(DT[dtype]).eps * want.abs() + 1e-2 + torch.nan_to_num(lost, nan=0.0, posinf=0.0)
+        assert ((got - want).abs() <= tol)[ok].all()
