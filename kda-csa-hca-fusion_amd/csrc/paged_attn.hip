@@ -6,14 +6,15 @@
 //   s = scale q^ K^T,  out = sum_k e^(s_k) K_k / (sum_k e^(s_k) + e^sink_h)
 // and 0 where no key is visible (/root/reference/ops_hca.py:132-194 over a cache,
 // /root/reference/ops_decoding_cache.py:1268-1395; chunks of one token are its
-// decode step). The query is rounded to 16 bits and so are the weights e^(s - M) in
-// the second product: to bf16, which has the range of fp32 that unnormalised queries
-// and rows scaled by any power of two need and holds the rows of every storage
-// format exactly; to fp16, finer by three bits, where the queries are fp16, for what
-// such a model's rows are fits it (paged.h). Scores, sums and outputs are fp32. The
-// second rounding of a bf16 query by itself is what leaves a bf16 output 0.0025
-// off where its own rounding leaves 0.0017 (both products in two parts would take the
-// tile kernel's issue time up by 40%).
+// decode step). The products take 16-bit operands: bf16, which has the range of fp32 that
+// unnormalised queries and rows scaled by any power of two need and holds the rows of
+// every storage format exactly; fp16, finer by three bits, where the queries are fp16, for
+// what such a model's rows are fits it (paged.h). Scores, sums and outputs are fp32.
+// A query enters as it is, times a power of two: what is left of 1 / ||q|| multiplies the
+// scores with the scale, so a 16-bit query is not rounded again (that alone took a bf16
+// output from 0.0020 off to 0.0026; its own rounding leaves 0.0017). The
+// weights e^(s - M) are rounded to the products' type in the second product, and fp32
+// queries, as the rest of the framework's attention does, to bf16.
 //
 // All heads share the keys (MQA), so the query rows of a sequence are its tokens
 // times its heads, nh rows a token, and a 16-row MFMA tile may hold rows of
@@ -134,6 +135,38 @@ __device__ __forceinline__ int computed_rows(const PagedAttnParams& p, const Pag
 template <typename T> struct Prod { typedef bf16_t type; };
 template <> struct Prod<_Float16> { typedef _Float16 type; };
 
+// MqaWave for queries of type T.
+template <int HD, typename T> struct PagedWave : MqaWave<HD, typename Prod<T>::type> {
+  typedef typename Prod<T>::type E;
+  typedef MqaWave<HD, E> Base;
+  // The query of this lane's row, at q_row (always readable; zeros where it is not `keep`).
+  // Normalised, it enters times the power of two of 1 / ||q||; the rest of that, in [1, 2),
+  // goes into the scores' factor. (1 / ||q|| of an infinite sum of squares is 0, and so is
+  // the query, its infinities NaN.)
+  __device__ __forceinline__ void query(const T* q_row, bool keep, bool normalise, float scale) {
+    const int q = lane_id() >> 4;
+    float f[Base::NS][8], ss = 0.f;
+#pragma unroll
+    for (int s = 0; s < Base::NS; ++s) {
+      Load8<T>::run(q_row + 32 * s + 8 * q, f[s]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        f[s][i] = keep ? f[s][i] : 0.f;
+        ss += f[s][i] * f[s][i];
+      }
+    }
+    const uint32_t inv = __float_as_uint(normalise ? l2_inv(colq_sum(ss)) : 1.f);
+    const float two = __uint_as_float(inv & 0x7f800000u), rest = __uint_as_float((inv & 0x7fffffu) | 0x3f800000u);
+#pragma unroll
+    for (int s = 0; s < Base::NS; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[s][i] *= two;
+    Base::setup(f, false, scale);
+    Base::qscale2 = fmaxf(fabsf(scale) * kLog2eF * rest, 1e-30f);
+    Base::thr = (kMFloor + kRescaleLog2) / Base::qscale2;
+  }
+};
+
 // Whether a lane of the wave holds a NaN.
 __device__ __forceinline__ bool any_nan(const float (&sc)[8]) {
   bool n = false;
@@ -179,7 +212,7 @@ template <int HD, int FMT, int QW, bool BIG, typename T>
 __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_token_kernel(PagedAttnParams p) {
   typedef typename Prod<T>::type E;
   typedef PagedKey<FMT, E> Key;
-  using W = MqaWave<HD, E>;
+  using W = PagedWave<HD, T>;
   typedef typename W::v8 v8;
   constexpr int ROWB = FMT == PF_BF16 ? 2 * HD : HD;  // bytes of a key row
   constexpr int TPR = ROWB / 16;                      // lanes per key row
@@ -295,8 +328,8 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
       const int rr = live ? r : nrow - 1;
       const int tok = rr / p.nh;
       head[u] = rr - tok * p.nh;
-      w[u].template init_always<T>(static_cast<const T*>(p.q) + ((long long)sq.row0 * p.nh + rr) * HD, live,
-                                   p.normalize_q != 0, p.scale / Key::held);
+      w[u].query(static_cast<const T*>(p.q) + ((long long)sq.row0 * p.nh + rr) * HD, live, p.normalize_q != 0,
+                 p.scale / Key::held);
       const uint32_t pos = sq.ctx + tok;
       const uint32_t f = pos + 1 > (uint32_t)p.win ? pos + 1 - p.win : 0;
       // (a padding row is never stored: it masks nothing)
@@ -494,7 +527,7 @@ template <int HD, int FMT, int RG, int QW, typename T>
 __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_kernel(PagedAttnParams p) {
   typedef typename Prod<T>::type E;
   typedef PagedKey<FMT, E> Key;
-  using W = MqaWave<HD, E>;
+  using W = PagedWave<HD, T>;
   typedef typename W::v8 v8;
   constexpr int NWV = RG / QW, NTH = 64 * NWV;
   constexpr int ROWS = 16 * RG;
@@ -630,7 +663,7 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
     const int tok = rr / p.nh;
     head[u] = rr - tok * p.nh;
     const T* qrow = static_cast<const T*>(p.q) + ((long long)sq.row0 * p.nh + rr) * HD;
-    w[u].template init_always<T>(qrow, live, p.normalize_q != 0, p.scale / Key::held);
+    w[u].query(qrow, live, p.normalize_q != 0, p.scale / Key::held);
     const RowKeys k = row_keys(p, sq, sp, tok, k1);
     // (a padding row is never stored: it masks nothing)
     vis[u] = live ? k.vis : k1;

@@ -140,6 +140,71 @@ def test_rows_with_a_channel_that_is_not_finite(dev, store, normalize, bad):
         assert torch.isnan(win[~ok]).all() and torch.isfinite(win[ok]).all() and (win[ok].abs().amax(-1) > 0).all()
 
 
+# --------------------------------------------------------------------------- bits kept
+
+# A rounding to a type whose half step is u is off by u / sqrt(3) sqrt(3 / (8 ln 2)) = 0.425 u of the value in the root
+# mean square (values spread evenly over their logarithm). An output has two of them, its own and those of
+# its weights, which for keys of random directions add up in norm as the weighted keys themselves do: 0.601 u
+# of the output's norm, 2.35e-3 in bf16 and 2.94e-4 in fp16. A query of 16 bits has none: one rounded once more
+# would move scores by 0.425 u |scale| / sqrt(c) in the root mean square, at |scale| = 64 and c = 128 seven
+# times those bounds (c = 64: ten times). fp32 queries: what is left are fp32 sums of at most c products and
+# the exponentials, a few 2^-24 of the scores' |scale| log2 e <= 93 and of the output: 16 2^-24 |scale| allowed.
+def rms_bound(dtype, scale):
+    u = {"bf16": 2.0 ** -8, "fp16": 2.0 ** -11}.get(dtype)
+    return 1.05 * 0.601 * u if u else 16 * 2.0 ** -24 * abs(scale)
+
+
+BITS = [
+    # lens, ctx, m2, win, nh, c, page, store
+    ([1], [5003], 128, 128, 16, 128, 16, "bf16"),
+    ([1, 1, 1], [40, 4095, 16383], 4, 77, 16, 128, 64, "e4m3"),
+    ([8, 1, 3, 5], [100, 0, 63, 8190], 64, 16, 4, 64, 32, "int8"),
+    ([4], [600], 16, 64, 16, 128, 64, "bf16"),
+    ([90, 17], [9000, 3000], 8, 33, 2, 128, 64, "e4m3"),
+    ([130, 1], [2000, 600], 16, 128, 16, 64, 32, "int8"),
+    ([30], [50000], 16, 128, 16, 128, 64, "bf16"),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -12, 37.0])
+@pytest.mark.parametrize("i", range(len(BITS)))
+def test_queries_keep_their_bits(dev, i, size, dtype):
+    """Normalised queries of any length, at a scale where a rounding of theirs would show."""
+    lens, ctx, m2, win, nh, c, page, store = BITS[i]
+    rng = np.random.default_rng(600 + i)
+    slots = list(rng.permutation(len(lens)))
+    pool = ref.Pool(len(lens), *pages_for(lens, ctx, m2, win, page), page, c, store, seed=i)
+    fill(pool, lens, ctx, slots, m2, win, rng)
+    q = torch.from_numpy(size * rng.standard_normal((sum(lens), nh, c))).to("cuda", DT[dtype])
+    for scale in (64.0, -64.0):
+        out = run_attention(pool, q, lens, ctx, slots, m2, win, None, scale)
+        want, _ = ref.attention(pool, f64(q), lens, ctx, slots, m2=m2, win=win, sink=None, scale=scale)
+        err = np.linalg.norm(f64(out) - want) / np.linalg.norm(want)
+        assert err <= rms_bound(dtype, scale), err
+
+
+def test_lengths_of_queries_past_the_sums(dev):
+    """Queries of zeros, of an infinite sum of squares (normalised to zeros, as F.normalize in fp32) and NaN."""
+    rng = np.random.default_rng(36)
+    m2, win, c, nh = 16, 32, 128, 4
+    for n in (4, 40):
+        pool = ref.Pool(1, *pages_for([n], [300], m2, win, 32), 32, c, "e4m3")
+        fill(pool, [n], [300], [0], m2, win, rng)
+        for dtype in ("bf16", "fp32"):
+            q = torch.from_numpy(rng.standard_normal((n, nh, c))).to("cuda", DT[dtype])
+            q[0] = 0.0
+            zero = run_attention(pool, q, [n], [300], [0], m2, win, None, 8.0)
+            q[0] = 1e30
+            big = run_attention(pool, q, [n], [300], [0], m2, win, None, 8.0)
+            assert torch.equal(big, zero) and torch.isfinite(big).all()
+            q[0, :, 3] = float("inf")
+            q[1, 2, 5] = float("nan")
+            out = run_attention(pool, q, [n], [300], [0], m2, win, None, 8.0)
+            assert torch.isnan(out[0]).all() and torch.isnan(out[1, 2]).all()
+            assert torch.equal(out[2:], big[2:]) and torch.equal(out[1, :2], big[1, :2])
+
+
 # --------------------------------------------------------------------------- 4-bit weights
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
