@@ -607,7 +607,8 @@ int kch_hca_paged_append(const void* C, long long ldc, const void* Z, long long 
  * NULL; normalize_q: L2-normalise the queries. max_ctx is at least the largest
  * ctx (it lays the work out; a larger one is answered rightly, if slower).
  * The products take bf16, with dtype fp16 fp16: rows with values past its range
- * then read as NaN (kept in 8 bits, past four times its range).
+ * then read as NaN (kept in 8 bits, past four times its range). With dtype fp32 they
+ * take three bf16 parts of the queries and of the weights, and keep fp32's accuracy.
  * Rows of out that no sequence answers (ahead of cu[0], behind cu[S], of a sequence
  * that is passed over, of a chunk past max_len) are left as they were, or zeros with
  * zero_tail. ws as kch_hca_paged_attn_ws_bytes says, 256-byte aligned.

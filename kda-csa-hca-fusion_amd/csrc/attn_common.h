@@ -292,8 +292,13 @@ struct MqaWave {
 
   // Softmax step over 32 keys: sc = this lane's raw scores of keys 4q..4q+3
   // and 16+4q..16+4q+3 (-inf = masked). Rescales o and L when a score moves
-  // M, adds the keys' p to L and returns p as the B operand of the O^T update.
+  // M, adds the keys' p to L and returns p (softmax32: as the B operand of the O^T
+  // update).
+  typedef float f32x8 __attribute__((ext_vector_type(8)));
   __device__ __forceinline__ v8 softmax32(const float (&sc)[8]) {
+    return __builtin_convertvector(weights32(sc), v8);
+  }
+  __device__ __forceinline__ f32x8 weights32(const float (&sc)[8]) {
     bool up = false;
 #pragma unroll
     for (int e = 0; e < 8; ++e) up |= sc[e] > thr;
@@ -309,13 +314,12 @@ struct MqaWave {
       M = mnew;
       thr = (mnew + kRescaleLog2) / qscale2;
     }
-    typedef float f32x8 __attribute__((ext_vector_type(8)));
     f32x8 pe;
     const float nm = -M;
 #pragma unroll
     for (int e = 0; e < 8; ++e) pe[e] = fast_exp2(fmaf(sc[e], qscale2, nm));
     L += ((pe[0] + pe[1]) + (pe[2] + pe[3])) + ((pe[4] + pe[5]) + (pe[6] + pe[7]));
-    return __builtin_convertvector(pe, v8);
+    return pe;
   }
 
   // V^T fragment t (16 dims x 32 keys) of 32 key rows in a swizzled LDS tile:

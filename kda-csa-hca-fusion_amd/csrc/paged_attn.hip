@@ -13,8 +13,11 @@
 // A query enters as it is, times a power of two: what is left of 1 / ||q|| multiplies the
 // scores with the scale, so a 16-bit query is not rounded again (that alone took a bf16
 // output from 0.0020 off to 0.0026; its own rounding leaves 0.0017). The
-// weights e^(s - M) are rounded to the products' type in the second product, and fp32
-// queries, as the rest of the framework's attention does, to bf16.
+// weights e^(s - M) are rounded to the products' type, as such queries' outputs are. An
+// fp32 query and its weights enter as the three bf16 parts that they are the sums of, three
+// products for one, and its output is off by what fp32 sums are (one bf16 part of each: 2e-3).
+// That takes 48 us a call where bf16 queries take 31 (128 tokens of a batch), 241 where they
+// take 115 (prompt chunks), and as long for short contexts.
 //
 // All heads share the keys (MQA), so the query rows of a sequence are its tokens
 // times its heads, nh rows a token, and a 16-row MFMA tile may hold rows of
@@ -135,10 +138,24 @@ __device__ __forceinline__ int computed_rows(const PagedAttnParams& p, const Pag
 template <typename T> struct Prod { typedef bf16_t type; };
 template <> struct Prod<_Float16> { typedef _Float16 type; };
 
-// MqaWave for queries of type T.
+// MqaWave for queries of type T. A product has kParts of them: an fp32 value is the sum of
+// three bf16 ones (hi + mid + lo, 24 significant bits), and the keys are one exactly.
 template <int HD, typename T> struct PagedWave : MqaWave<HD, typename Prod<T>::type> {
   typedef typename Prod<T>::type E;
   typedef MqaWave<HD, E> Base;
+  typedef typename Base::v8 v8;
+  typedef typename Base::f32x8 f32x8;
+  static constexpr int kParts = __is_same(T, float) ? 3 : 1;
+  v8 qx[kParts > 1 ? kParts - 1 : 1][Base::NS];  // mid and lo (hi: qf)
+
+  // x's bf16 parts, the largest first.
+  static __device__ __forceinline__ void parts(f32x8 x, v8 (&p)[kParts]) {
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      p[i] = __builtin_convertvector(x, v8);
+      if (i + 1 < kParts) x -= __builtin_convertvector(p[i], f32x8);
+    }
+  }
   // The query of this lane's row, at q_row (always readable; zeros where it is not `keep`).
   // Normalised, it enters times the power of two of 1 / ||q||; the rest of that, in [1, 2),
   // goes into the scores' factor. (1 / ||q|| of an infinite sum of squares is 0, and so is
@@ -157,13 +174,38 @@ template <int HD, typename T> struct PagedWave : MqaWave<HD, typename Prod<T>::t
     }
     const uint32_t inv = __float_as_uint(normalise ? l2_inv(colq_sum(ss)) : 1.f);
     const float two = __uint_as_float(inv & 0x7f800000u), rest = __uint_as_float((inv & 0x7fffffu) | 0x3f800000u);
-#pragma unroll
-    for (int s = 0; s < Base::NS; ++s)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[s][i] *= two;
-    Base::setup(f, false, scale);
+    Base::setup(f, false, 0.f);
     Base::qscale2 = fmaxf(fabsf(scale) * kLog2eF * rest, 1e-30f);
     Base::thr = (kMFloor + kRescaleLog2) / Base::qscale2;
+#pragma unroll
+    for (int s = 0; s < Base::NS; ++s) {
+      f32x8 x;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = f[s][i] * (scale < 0.f ? -two : two);
+      v8 p[kParts];
+      parts(x, p);
+      Base::qf[s] = p[0];
+#pragma unroll
+      for (int i = 1; i < kParts; ++i) qx[i - 1][s] = p[i];
+    }
+  }
+  __device__ __forceinline__ void nothing() {
+    float z[Base::NS][8] = {};
+    Base::setup(z, false, 1.f);
+  }
+  // S^T accumulator of 16 key rows, the least part first.
+  __device__ __forceinline__ f32x4 scores(const v8 (&k)[Base::NS]) const {
+    f32x4 st = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = kParts - 1; i >= 0; --i)
+#pragma unroll
+      for (int s = 0; s < Base::NS; ++s) st = Mfma16<E>::run(k[s], i ? qx[i ? i - 1 : 0][s] : Base::qf[s], st);
+    return st;
+  }
+  __device__ __forceinline__ void softmax(const float (&sc)[8], v8 (&p)[kParts]) { parts(Base::weights32(sc), p); }
+  __device__ __forceinline__ void add(int t, v8 v, const v8 (&p)[kParts]) {
+#pragma unroll
+    for (int i = kParts - 1; i >= 0; --i) Base::o[t] = Mfma16<E>::run(v, p[i], Base::o[t]);
   }
 };
 
@@ -205,11 +247,12 @@ __device__ __forceinline__ void store_group(const PagedAttnParams& p, const MqaW
 // branch (a wait there would drain every load in flight): past the end the last
 // step is read again.
 // Workgroups a CU at least (as many as leave registers for a step in flight without spilling).
-constexpr int token_min_blocks(int HD, int FMT, int QW) {
-  return (QW == 1 ? 3 : 2) - (HD == 128 && FMT == PF_BF16 ? 1 : 0);
+constexpr int token_min_blocks(int HD, int FMT, int QW, bool f32) {
+  const int n = (QW == 1 ? 3 : 2) - (HD == 128 && FMT == PF_BF16 ? 1 : 0);
+  return f32 && n > 1 ? n - 1 : n;
 }
 template <int HD, int FMT, int QW, bool BIG, typename T>
-__global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_token_kernel(PagedAttnParams p) {
+__global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW, __is_same(T, float))) void paged_token_kernel(PagedAttnParams p) {
   typedef typename Prod<T>::type E;
   typedef PagedKey<FMT, E> Key;
   using W = PagedWave<HD, T>;
@@ -412,7 +455,7 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
           else rb[u] = w[u].scores(kf);
         }
       }
-      v8 pb8[QW];
+      v8 pb8[QW][W::kParts];
       bool holes = false;  // a NaN that some row does not see
 #pragma unroll
       for (int u = 0; u < QW; ++u) {
@@ -430,7 +473,7 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
             sc[e] = j >= la && j < lb ? sc[e] : -INFINITY;
           }
         }
-        pb8[u] = w[u].softmax32(sc);
+        w[u].softmax(sc, pb8[u]);
       }
 #pragma unroll
       for (int t0 = 0; t0 < W::NT; t0 += 4) {
@@ -444,7 +487,7 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int u = 0; u < QW; ++u) w[u].o[t0 + t] = Mfma16<E>::run(va[t], pb8[u], w[u].o[t0 + t]);
+          for (int u = 0; u < QW; ++u) w[u].add(t0 + t, va[t], pb8[u]);
       }
     };
 
@@ -458,8 +501,7 @@ __global__ __launch_bounds__(256, token_min_blocks(HD, FMT, QW)) void paged_toke
   } else {
 #pragma unroll
     for (int u = 0; u < QW; ++u) {
-      float z[W::NS][8] = {};
-      w[u].setup(z, false, 1.f);
+      w[u].nothing();
       head[u] = 0;
     }
   }
@@ -524,7 +566,7 @@ __device__ __forceinline__ RowKeys row_keys(const PagedAttnParams& p, const Page
 // takes 71 for 16 chunks without a context, 167 where it takes 143 on bf16 rows (125 us
 // for this one then).
 template <int HD, int FMT, int RG, int QW, typename T>
-__global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_kernel(PagedAttnParams p) {
+__global__ __launch_bounds__(64 * (RG / QW), RG == 8 && !__is_same(T, float) ? 4 : 2) void paged_attn_kernel(PagedAttnParams p) {
   typedef typename Prod<T>::type E;
   typedef PagedKey<FMT, E> Key;
   using W = PagedWave<HD, T>;
@@ -694,7 +736,7 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
         else sb[u] = w[u].scores(kf);
       }
     }
-    v8 pb[QW];
+    v8 pb[QW][W::kParts];
     bool holes = false;  // a NaN that some row does not see
 #pragma unroll
     for (int u = 0; u < QW; ++u) {
@@ -712,7 +754,7 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
           sc[e] = ok ? sc[e] : -INFINITY;
         }
       }
-      pb[u] = w[u].softmax32(sc);
+      w[u].softmax(sc, pb[u]);
     }
     // a wave at its products goes before those at their softmax (8 short-context chunks
     // 82.6 -> 76.8 us, long ones 126 -> 122)
@@ -729,7 +771,7 @@ __global__ __launch_bounds__(64 * (RG / QW), RG == 8 ? 4 : 2) void paged_attn_ke
 #pragma unroll
       for (int t = 0; t < kPv; ++t)
 #pragma unroll
-        for (int u = 0; u < QW; ++u) w[u].o[t0 + t] = Mfma16<E>::run(va[t], pb[u], w[u].o[t0 + t]);
+        for (int u = 0; u < QW; ++u) w[u].add(t0 + t, va[t], pb[u]);
     }
     __builtin_amdgcn_s_setprio(0);
   };

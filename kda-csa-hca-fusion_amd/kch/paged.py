@@ -188,7 +188,7 @@ def hca_paged_attention(q, rows, scales, block_table, ring_table, slots, cu_seql
     sequence that is passed over (a slot outside the table, as a padding entry has it, a negative
     context, rows outside ``q``).
     The products are bf16 with fp32 sums, for fp16 ``q`` fp16: there a row with values past
-    fp16's range reads as NaN.
+    fp16's range reads as NaN. For fp32 ``q`` they take three bf16 parts, which keep fp32's accuracy.
     """
     fn = "hca_paged_attention"
     fmt, dev, P, page, c, n_slots, nbp, nrp, S = _step(fn, rows, scales, block_table, ring_table, slots,

@@ -166,7 +166,7 @@ BITS = [
 ]
 
 
-@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("size", [1.0, 2.0 ** -12, 37.0])
 @pytest.mark.parametrize("i", range(len(BITS)))
 def test_queries_keep_their_bits(dev, i, size, dtype):
@@ -182,6 +182,21 @@ def test_queries_keep_their_bits(dev, i, size, dtype):
         want, _ = ref.attention(pool, f64(q), lens, ctx, slots, m2=m2, win=win, sink=None, scale=scale)
         err = np.linalg.norm(f64(out) - want) / np.linalg.norm(want)
         assert err <= rms_bound(dtype, scale), err
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_fp32_queries_that_are_not_normalised(dev, n):
+    rng = np.random.default_rng(35)
+    m2, win, c, nh = 16, 32, 128, 16
+    pool = ref.Pool(1, *pages_for([n], [700], m2, win, 32), 32, c, "bf16")
+    fill(pool, [n], [700], [0], m2, win, rng, scale_rows=3.0)
+    q = torch.from_numpy(rng.standard_normal((n, nh, c))).float().cuda()
+    snk = rng.standard_normal(nh).astype(np.float32)
+    out = run_attention(pool, q, [n], [700], [0], m2, win, snk, c ** -0.5, normalize_q=False)
+    want, _ = ref.attention(pool, f64(q), [n], [700], [0], m2=m2, win=win, sink=snk, scale=c ** -0.5,
+                            normalize_q=False)
+    # scores of up to 3 |q| / sqrt(c) = 4: as |scale| = 4 of unit vectors
+    assert np.linalg.norm(f64(out) - want) <= 16 * 2.0 ** -24 * 4 * np.linalg.norm(want)
 
 
 def test_lengths_of_queries_past_the_sums(dev):
