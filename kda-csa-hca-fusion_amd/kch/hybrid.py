@@ -760,11 +760,14 @@ class HCAHybridLayer(_FusedWeightLayer):
         of the sequences ``slots`` of ``cache``, packed rows ``x`` ``[N, d]``; what ``forward``
         gives at these positions of the whole sequences. ``residual`` is added.
         ``weight_group`` 32, 64 or 128: the projections run on 4-bit copies of the weights
-        with groups of so many columns (bf16 or fp16 ``x``), made once. Forward only."""
+        with groups of so many columns (bf16 or fp16 ``x``), made once. Forward only: inputs
+        that ask for gradients are refused, the layer's own weights are constants."""
         cfg = self.cfg
         c, nh, dc = cfg.hca_c, cfg.hca_nh, cfg.hca_dc
         if x.dim() != 2 or x.shape[1] != cfg.d_model:
             raise ValueError(f"forward_paged: x must be [N, {cfg.d_model}], got {tuple(x.shape)}")
+        if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+            raise NotImplementedError("forward_paged: no gradients (call it under torch.no_grad())")
         proj = [self.W_KV.weight, self.W_Z.weight, self.W_DQ.weight]
         with torch.no_grad():
             w_in, w_up, B_pos, sink = self._step_weights(x.dtype, x.device)

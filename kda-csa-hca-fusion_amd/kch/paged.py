@@ -365,6 +365,7 @@ class HCAPagedCache:
         ``C_new, Z_new`` ``[sum(lens), c]``, packed in that order."""
         fn = "append_step"
         self._eager(fn)
+        _no_grad(f"HCAPagedCache.{fn}", C_new, Z_new, B_pos)
         slots = list(slots)
         lens = [1] * len(slots) if lens is None else list(lens)
         if len(lens) != len(slots) or len(set(slots)) != len(slots):
@@ -414,6 +415,7 @@ class HCAPagedCache:
         """``[N, nh, c]`` in ``q.dtype``: the queries of the last ``append_step``'s tokens."""
         fn = "HCAPagedCache.forward_step"
         self._eager("forward_step")
+        _no_grad(fn, q, sink_logits)
         if self._last is None:
             _fail(fn, "append_step first")
         _, slots, cu, ctx, n, max_len, max_ctx = self._last

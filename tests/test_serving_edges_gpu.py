@@ -220,6 +220,44 @@ def test_lengths_of_queries_past_the_sums(dev):
             assert torch.equal(out[2:], big[2:]) and torch.equal(out[1, :2], big[1, :2])
 
 
+# --------------------------------------------------------------------------- the class and the layer
+
+def test_class_and_layer_refuse_inputs_that_ask_for_gradients(dev):
+    import kch
+    cache = kch.HCAPagedCache(8, 64, 8, 8, max_seqs=1, max_tokens=64, max_chunk=4, page=16)
+    s = cache.add()
+    x, Bp = torch.ones(1, 64, device="cuda"), torch.zeros(8, 64, device="cuda")
+    ask = lambda t: t.clone().requires_grad_()  # noqa: E731
+    for args in ((ask(x), x, Bp), (x, ask(x), Bp), (x, x, ask(Bp))):
+        with pytest.raises(NotImplementedError, match="no gradients"):
+            cache.append_step([s], *args)
+    assert cache.n_tokens(s) == 0
+    with torch.no_grad():
+        cache.append_step([s], ask(x), x, ask(Bp))
+        want = cache.forward_step(ask(x)[:, None])
+    with pytest.raises(NotImplementedError, match="no gradients"):
+        cache.forward_step(ask(x)[:, None])
+    with pytest.raises(NotImplementedError, match="no gradients"):
+        cache.forward_step(x[:, None], sink_logits=torch.zeros(1, device="cuda", requires_grad=True))
+    assert torch.equal(cache.forward_step(x[:, None]), want)
+
+    cfg = kch.HybridConfig(d_model=128, hca_m2=16, hca_nh=2, hca_c=64, hca_dc=64, hca_sliding_window=24)
+    layer = kch.HCAHybridLayer(cfg).cuda().bfloat16()
+    served = layer.paged_cache(8, max_seqs=1, max_tokens=64, max_chunk=4, page=16)
+    t = served.add()
+    x = torch.randn(1, 128, device="cuda").bfloat16()
+    for group in (0, 64):
+        for kw in (dict(x=ask(x)), dict(x=x, residual=ask(x))):
+            with pytest.raises(NotImplementedError, match="no gradients"):
+                layer.forward_paged(kw.pop("x"), served, [t], weight_group=group, **kw)
+        assert served.n_tokens(t) == 0
+    # the layer's own weights are constants to it
+    assert not layer.forward_paged(x, served, [t]).requires_grad
+    with torch.no_grad():
+        layer.forward_paged(ask(x), served, [t], residual=ask(x))
+    assert served.n_tokens(t) == 2
+
+
 # --------------------------------------------------------------------------- 4-bit weights
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
