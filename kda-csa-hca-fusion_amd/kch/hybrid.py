@@ -768,6 +768,11 @@ class HCAHybridLayer(_FusedWeightLayer):
             raise ValueError(f"forward_paged: x must be [N, {cfg.d_model}], got {tuple(x.shape)}")
         if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
             raise NotImplementedError("forward_paged: no gradients (call it under torch.no_grad())")
+        # (the operators' own checks see one tensor's sizes at a time: not the window, nor how rows are held)
+        if (cache.c, cache.m2, cache.win, cache.normalize_qk) != (c, cfg.hca_m2, cfg.hca_sliding_window, True):
+            raise ValueError(f"forward_paged: the cache has c={cache.c}, m2={cache.m2}, win={cache.win}, "
+                             f"normalize_qk={cache.normalize_qk}, the layer c={c}, m2={cfg.hca_m2}, "
+                             f"win={cfg.hca_sliding_window} and normalised rows")
         proj = [self.W_KV.weight, self.W_Z.weight, self.W_DQ.weight]
         with torch.no_grad():
             w_in, w_up, B_pos, sink = self._step_weights(x.dtype, x.device)

@@ -258,6 +258,23 @@ def test_class_and_layer_refuse_inputs_that_ask_for_gradients(dev):
     assert served.n_tokens(t) == 2
 
 
+def test_layer_refuses_a_cache_of_another_kind(dev):
+    """A window or rows of another kind than its forward's would answer something else."""
+    import kch
+    cfg = kch.HybridConfig(d_model=128, hca_m2=16, hca_nh=2, hca_c=64, hca_dc=64, hca_sliding_window=24)
+    layer = kch.HCAHybridLayer(cfg).cuda().bfloat16()
+    x = torch.randn(1, 128, device="cuda").bfloat16()
+    for c, m2, win, kw in ((64, 16, 8, {}), (64, 16, 0, {}), (64, 8, 24, {}), (32, 16, 24, {}),
+                           (64, 16, 24, dict(normalize_qk=False))):
+        cache = kch.HCAPagedCache(8, c, m2, win, max_seqs=1, max_tokens=64, page=32, **kw)
+        s = cache.add()
+        with pytest.raises(ValueError, match="forward_paged: the cache"):
+            layer.forward_paged(x, cache, [s])
+        assert cache.n_tokens(s) == 0
+    cache = kch.HCAPagedCache(8, 64, 16, 24, max_seqs=1, max_tokens=64, page=32)
+    assert layer.forward_paged(x, cache, [cache.add()]).shape == x.shape
+
+
 # --------------------------------------------------------------------------- 4-bit weights
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
