@@ -775,17 +775,20 @@ class HCAHybridLayer(_FusedWeightLayer):
                              f"win={cfg.hca_sliding_window} and normalised rows")
         proj = [self.W_KV.weight, self.W_Z.weight, self.W_DQ.weight]
         with torch.no_grad():
-            w_in, w_up, B_pos, sink = self._step_weights(x.dtype, x.device)
             if weight_group:
+                # (_step_weights would keep 16-bit copies that nothing reads)
+                wide, small = [self.W_UQ.weight, self.o_proj.weight], [self.B_pos, self.sink]
+
                 def build():
-                    ws = [torch.cat([p.detach() for p in proj], 0), self.W_UQ.weight, self.o_proj.weight]
-                    return [quantize_w4(w.to(x.device), weight_group, dtype=x.dtype) for w in ws]
+                    ws = [torch.cat([p.detach() for p in proj], 0)] + wide
+                    return [quantize_w4(w.to(x.device), weight_group, dtype=x.dtype) for w in ws] + \
+                        [p.detach().to(device=x.device, dtype=torch.float32).contiguous() for p in small]
                 fused = self._fused_w4.setdefault(weight_group, _FusedWeight())
-                w_in, w_up, w_out = fused.get(proj + [self.W_UQ.weight, self.o_proj.weight], x.dtype,
-                                              x.device, build)
+                w_in, w_up, w_out, B_pos, sink = fused.get(proj + wide + small, x.dtype, x.device, build)
                 C, Z, cQ = linear_w4(x, *w_in).split([c, c, dc], -1)
                 q = linear_w4(cQ, *w_up)
             else:
+                w_in, w_up, B_pos, sink = self._step_weights(x.dtype, x.device)
                 C, Z, cQ = _linear(x, w_in).split([c, c, dc], -1)
                 q = _linear(cQ, w_up)
             cache.append_step(slots, C, Z, B_pos, lens)

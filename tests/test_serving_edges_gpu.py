@@ -275,6 +275,25 @@ def test_layer_refuses_a_cache_of_another_kind(dev):
     assert layer.forward_paged(x, cache, [cache.add()]).shape == x.shape
 
 
+def test_four_bit_serving_holds_no_16_bit_copies(dev):
+    import kch
+    cfg = kch.HybridConfig(d_model=1024, hca_m2=16, hca_nh=16, hca_c=64, hca_dc=512, hca_sliding_window=24)
+    layer = kch.HCAHybridLayer(cfg).cuda().bfloat16()
+    cache = layer.paged_cache(8, max_seqs=1, max_tokens=64, page=32)
+    s = cache.add()
+    x = torch.randn(1, 1024, device="cuda").bfloat16()
+    layer.forward_paged(x, cache, [s], weight_group=64)   # (the codes are made here)
+    layer.invalidate_weight_cache()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    layer.forward_paged(x, cache, [s], weight_group=64)
+    held = torch.cuda.memory_allocated() - before
+    n = sum(p.numel() for p in (layer.W_KV.weight, layer.W_Z.weight, layer.W_DQ.weight, layer.W_UQ.weight,
+                                layer.o_proj.weight))
+    # codes, 16-bit scales and zero points a group, small vectors and the allocator's steps
+    assert held <= n / 2 + 3 * n / 64 + 2 ** 18, (held, n)
+
+
 # --------------------------------------------------------------------------- 4-bit weights
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
