@@ -102,6 +102,14 @@ def _linear_residual(x: torch.Tensor, w: torch.Tensor, residual: torch.Tensor) -
     return out.view(residual.shape)
 
 
+def _broadcasts(a, b) -> bool:
+    try:
+        torch.broadcast_shapes(a, b)
+    except RuntimeError:
+        return False
+    return True
+
+
 def _grad_wanted(*ts) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
@@ -773,6 +781,15 @@ class HCAHybridLayer(_FusedWeightLayer):
             raise ValueError(f"forward_paged: the cache has c={cache.c}, m2={cache.m2}, win={cache.win}, "
                              f"normalize_qk={cache.normalize_qk}, the layer c={c}, m2={cfg.hca_m2}, "
                              f"win={cfg.hca_sliding_window} and normalised rows")
+        # what the last product would refuse, before the tokens are in the cache
+        if residual is not None:
+            fits = residual.shape == x.shape and residual.dtype is x.dtype if weight_group else \
+                _broadcasts(residual.shape, x.shape)
+            if not fits or residual.device != x.device:
+                raise ValueError(f"forward_paged: residual must be {tuple(x.shape)} {x.dtype} on {x.device}, got "
+                                 f"{tuple(residual.shape)} {residual.dtype} on {residual.device}")
+        if not weight_group and self.o_proj.weight.dtype != x.dtype and not torch.is_autocast_enabled():
+            raise TypeError(f"forward_paged: x is {x.dtype}, the layer's weights {self.o_proj.weight.dtype}")
         proj = [self.W_KV.weight, self.W_Z.weight, self.W_DQ.weight]
         with torch.no_grad():
             if weight_group:

@@ -275,6 +275,28 @@ def test_layer_refuses_a_cache_of_another_kind(dev):
     assert layer.forward_paged(x, cache, [cache.add()]).shape == x.shape
 
 
+def test_layer_refuses_before_the_tokens_are_appended(dev):
+    """A call that fails leaves the sequences as they were: the same tokens can be sent again."""
+    import kch
+    cfg = kch.HybridConfig(d_model=128, hca_m2=16, hca_nh=2, hca_c=64, hca_dc=64, hca_sliding_window=24)
+    layer = kch.HCAHybridLayer(cfg).cuda().bfloat16()
+    cache = layer.paged_cache(8, max_seqs=1, max_tokens=64, max_chunk=4, page=32)
+    s = cache.add()
+    x = torch.randn(2, 128, device="cuda").bfloat16()
+    for group, res in ((0, x[:, :64]), (0, x[None, :1, :64]), (0, x.repeat(2, 1)), (0, x.cpu()), (64, x[:1]), (64, x.float()),
+                       (64, x.cpu())):
+        with pytest.raises((ValueError, TypeError), match="residual"):
+            layer.forward_paged(x, cache, [s], [2], residual=res, weight_group=group)
+        assert cache.n_tokens(s) == 0, (group, res.shape)
+    with pytest.raises(TypeError, match="weights"):
+        layer.forward_paged(x.half(), cache, [s], [2])
+    with pytest.raises(TypeError, match="bfloat16"):
+        layer.forward_paged(x.float(), cache, [s], [2], weight_group=64)
+    assert cache.n_tokens(s) == 0
+    a = layer.forward_paged(x, cache, [s], [2], residual=x[:1])   # (broadcasts where no kernel adds it)
+    assert a.shape == x.shape and cache.n_tokens(s) == 2
+
+
 def test_four_bit_serving_holds_no_16_bit_copies(dev):
     import kch
     cfg = kch.HybridConfig(d_model=1024, hca_m2=16, hca_nh=16, hca_c=64, hca_dc=512, hca_sliding_window=24)
