@@ -292,15 +292,22 @@ class _FusedWeight:
     Writes through ``param.data`` (``p.data.copy_(...)``, EMA or weight-swap
     code) change neither the storage nor the autograd version counter: after
     such a write call the owning layer's ``invalidate_weight_cache()``.
-    ``load_state_dict`` and ``.to()`` / ``.half()`` invalidate by themselves."""
+    ``load_state_dict`` and ``.to()`` / ``.half()`` invalidate by themselves.
+
+    The storages that the copy was made from are held until it is made again: a
+    parameter that takes a freed one's place in memory, at its version, would
+    pass for it. A copied or pickled layer makes its own."""
 
     def __init__(self):
-        self._key = None
-        self._w = None
+        self.invalidate()
+
+    def __reduce__(self):
+        return (_FusedWeight, ())
 
     def invalidate(self):
         self._key = None
         self._w = None
+        self._held = None
 
     def get(self, params, dtype, device, build=None):
         """The row-concatenation of ``params`` in ``dtype`` on ``device``, or
@@ -310,6 +317,7 @@ class _FusedWeight:
         if key != self._key:
             self._w = (torch.cat([p.detach() for p in params], 0).to(device=device, dtype=dtype)
                        if build is None else build())
+            self._held = [None if p is None else p.detach() for p in params]
             self._key = key
         return self._w
 

@@ -3,6 +3,8 @@ lowest value, rows that are not finite, and how many bits the products keep."""
 
 from __future__ import annotations
 
+import copy
+
 import numpy as np
 import paged_ref as ref
 import pytest
@@ -314,6 +316,32 @@ def test_four_bit_serving_holds_no_16_bit_copies(dev):
                                 layer.o_proj.weight))
     # codes, 16-bit scales and zero points a group, small vectors and the allocator's steps
     assert held <= n / 2 + 3 * n / 64 + 2 ** 18, (held, n)
+
+
+@pytest.mark.parametrize("group", [0, 64])
+def test_weights_put_where_freed_ones_were(dev, group):
+    """A parameter replaced twice between two calls lies where the first one was: its copies are made anew."""
+    import kch
+    cfg = kch.HybridConfig(d_model=1024, hca_m2=16, hca_nh=16, hca_c=64, hca_dc=512, hca_sliding_window=24)
+    layer = kch.HCAHybridLayer(cfg).cuda().bfloat16()
+    x = torch.randn(1, 1024, device="cuda").bfloat16()
+
+    def first_token():
+        cache = layer.paged_cache(8, max_seqs=1, max_tokens=64, page=32)
+        return layer.forward_paged(x, cache, [cache.add()], weight_group=group)
+
+    def fresh():
+        return torch.nn.Parameter(torch.randn(layer.W_KV.weight.shape, device="cuda", dtype=torch.bfloat16))
+
+    layer.W_KV.weight = fresh()
+    first_token()
+    for _ in range(2):
+        layer.W_KV.weight = fresh()
+    got = first_token()
+    layer.invalidate_weight_cache()
+    assert torch.equal(got, first_token())
+    twin = copy.deepcopy(layer)  # makes its own copies
+    assert all(f._w is None for f in [twin._fused, twin._fused_step, *twin._fused_w4.values()])
 
 
 # --------------------------------------------------------------------------- 4-bit weights
