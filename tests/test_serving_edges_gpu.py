@@ -222,6 +222,65 @@ def test_lengths_of_queries_past_the_sums(dev):
             assert torch.equal(out[2:], big[2:]) and torch.equal(out[1, :2], big[1, :2])
 
 
+# --------------------------------------------------------------------------- long contexts
+
+LONG = [
+    # lens, ctx, m2, win, nh, c, page, store
+    ([1, 1, 1], [40, 4095, 7003], 1, 77, 16, 128, 64, "e4m3"),
+    ([1], [49999], 4, 128, 16, 128, 16, "bf16"),
+    ([2, 1], [7999, 6001], 1, 5, 16, 128, 32, "int8"),
+    ([3, 1], [24003, 100], 4, 16, 4, 64, 1, "int8"),
+    ([4], [12001], 1, 33, 16, 128, 64, "e4m3"),
+    ([130, 7], [9001, 3000], 1, 128, 1, 128, 32, "bf16"),
+    ([40, 30], [48000, 9], 4, 7, 4, 128, 64, "e4m3"),
+    ([17], [6200], 1, 16, 6, 64, 128, "int8"),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("i", range(len(LONG)))
+def test_every_key_counts_once(dev, i, dtype):
+    """Keys that are one unit vector each and queries of zeros: every channel of an output is how many keys have it
+    over how many there are, at most 110 here: a key left out or taken twice, at a border of ranges, steps, tiles
+    or pages, shows (one in 110 against half a step of 2^-8 and the fp32 sums)."""
+    lens, ctx, m2, win, nh, c, page, store = LONG[i]
+    rng = np.random.default_rng(700 + i)
+    slots = list(rng.permutation(len(lens)))
+    pool = ref.Pool(len(lens), *pages_for(lens, ctx, m2, win, page), page, c, store, seed=i)
+    most = 0
+    for slot, n, x in zip(slots, lens, ctx):
+        nb, pos = (x + n) // m2, np.arange(max(0, x - win + 1), x + n)
+        for table, at in ((pool.blocks, np.arange(nb)), (pool.ring, pos % pool.cap)):
+            # channels in turn, the turn's start by the slot
+            pool.put(table, slot, at, np.eye(c)[(np.arange(len(at)) * 7 + slot + (table is pool.ring)) % c])
+        most = max(most, -(-nb // c) + -(-win // c))
+    assert most <= 110
+    q = torch.zeros(sum(lens), nh, c, device="cuda", dtype=DT[dtype])
+    out = f64(run_attention(pool, q, lens, ctx, slots, m2, win, None, 8.0))
+    want, _ = ref.attention(pool, np.zeros(q.shape), lens, ctx, slots, m2=m2, win=win, sink=None, scale=8.0)
+    pos = np.concatenate([x + np.arange(n) for n, x in zip(lens, ctx)])
+    seen = ((pos + 1) // m2 + np.minimum(pos + 1, win))[:, None, None]
+    assert (np.abs(want * seen - np.rint(want * seen)) < 1e-6).all()
+    assert (np.abs(out * seen - want * seen) < 0.45).all(), np.abs(out * seen - want * seen).max()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("i", range(len(LONG)))
+def test_long_contexts_in_norm(dev, i, dtype):
+    """Random keys, the error against the output's norm: a step of keys left out would be several per cent."""
+    lens, ctx, m2, win, nh, c, page, store = LONG[i]
+    rng = np.random.default_rng(800 + i)
+    slots = list(rng.permutation(len(lens)))
+    pool = ref.Pool(len(lens), *pages_for(lens, ctx, m2, win, page), page, c, store, seed=i)
+    fill(pool, lens, ctx, slots, m2, win, rng)
+    q = torch.from_numpy(rng.standard_normal((sum(lens), nh, c))).to("cuda", DT[dtype])
+    snk = rng.standard_normal(nh).astype(np.float32)
+    out = run_attention(pool, q, lens, ctx, slots, m2, win, snk, 11.3)
+    want, _ = ref.attention(pool, f64(q), lens, ctx, slots, m2=m2, win=win, sink=snk, scale=11.3)
+    err = np.linalg.norm(f64(out) - want) / np.linalg.norm(want)
+    assert err <= rms_bound(dtype, 11.3), err
+
+
 # --------------------------------------------------------------------------- the class and the layer
 
 def test_class_and_layer_refuse_inputs_that_ask_for_gradients(dev):
@@ -390,3 +449,21 @@ def test_linear_w4_of_rows_that_are_not_finite(dev, dtype, M, N, K, G, zeros):
             lost = torch.from_numpy(K * 2.0 ** -53 * (np.abs(W) @ np.abs(xs)))
         tol = 2 * torch.finfo(DT[dtype]).eps * want.abs() + 1e-2 + torch.nan_to_num(lost, nan=0.0, posinf=0.0)
         assert ((got - want).abs() <= tol)[ok].all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("M,N,K,G,zeros", [
+    # 512 tiles of 16 x 16 and more: two and four of them a workgroup, N no multiple of theirs, tails of K
+    (3, 8212, 160, 32, True), (16, 8196, 256, 128, False), (33, 8212, 256, 128, True), (7, 8180, 192, 64, True),
+    (16, 16404, 96, 32, True), (5, 16404, 192, 64, False), (1, 16388, 160, 32, False), (20, 8260, 224, 32, True),
+    (9, 16372, 384, 128, True), (2, 8191, 160, 32, True),
+])
+def test_linear_w4_of_many_tiles(dev, dtype, residual, M, N, K, G, zeros):
+    import kch
+    from test_w4_gpu import check, make
+    w = make(N, K, G, zeros, dtype, M + N)
+    g = torch.Generator(device="cuda").manual_seed(K)
+    x = torch.randn(M, K, device="cuda", generator=g).to(DT[dtype])
+    res = torch.randn(M, N, device="cuda", generator=g).to(DT[dtype]) if residual else None
+    check(kch.linear_w4(x, *w, residual=res), x, *w, G, dtype, res)
