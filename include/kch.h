@@ -560,7 +560,8 @@ int kch_linear_up(const void* x, long long ldx, const void* w, long long ldw, vo
  *   rows [P, page, c]      the pool, page a power of two up to 1024, c 64 or
  *                          128, in `format`: 0 bf16, 1 e4m3 (OCP, no infinity), 2 int8
  *   scales [P, page]       8-bit formats: E8M0 codes of the rows' scales, value
- *                          = code 2^(scale code - 127); 255: the row is NaN
+ *                          = code 2^(scale code - 127), codes 1 to 254; 255: the row
+ *                          is NaN
  *   block_table [n_slots, nbp]  int32 page of a slot's compressed row b: entry
  *                          b / page, line b % page
  *   ring_table [n_slots, nrp]   int32 pages of its window rows: position p is

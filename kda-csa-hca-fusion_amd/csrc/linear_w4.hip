@@ -4,7 +4,9 @@
 // x's type; z uint8, or 8 everywhere. x and y bf16 or fp16, sums fp32, rounded once.
 //
 // It serves the layer projections of a decode step, as kch_linear_rows does, with a
-// quarter of the bytes; what bounds it is the stream of the codes.
+// quarter of the bytes; what bounds it is the stream of the codes. Every 16 rows read and unpack
+// them again: 64 rows of N 16384, K 8192 take 65 us where the bf16 product takes 47, 512 475
+// and 116 (N = K = 2048: 8.5 and 19, 25 and 20).
 //
 // y^T = W x^T on v_mfma_f32_16x16x32: A is a 16-row tile of W, B x^T (zero past
 // M). A code becomes a 16-bit float without arithmetic: the nibble in the low
@@ -93,7 +95,7 @@ template <int NT, int G> struct W4Piece {
 // bound the kernel (16 rows, N 4096, K 8192: 13.7 against 10.1 us). VEC: N is a multiple of 4,
 // four scales are one load. The loop has no load behind a branch: a wait there would drain
 // every load in flight (the same kernel with such loads took 145 us where it took 43).
-// At 16 rows, N 16384, K 8192 18.6 us, 3.8 TB/s; 13.9 us is what its 71 MB take at the rate of a
+// At 16 rows, N 16384, K 8192 17.3 us a call (traced 19.1 to 19.4), 4.1 TB/s; 13.9 us is what its 71 MB take at the rate of a
 // large copy. Past the stream it is the 56 vector instructions a tile and 128 k, mostly the
 // codes' unpacking.
 template <typename T, int NT, int KW, int G, bool ZP, bool VEC, bool KT>

@@ -55,7 +55,7 @@ __device__ __forceinline__ float amax_nan(float a, float x) {
 template <int FMT>
 __device__ __forceinline__ uint32_t quant4(float a, float b, float c, float d, int code) {
   if (code == kScaleNan) return 0u;
-  const float f = __uint_as_float((uint32_t)(254 - code) << 23);  // 2^(127 - code); 19 <= code <= 248
+  const float f = __uint_as_float((uint32_t)(254 - code) << 23);  // 2^(127 - code); 19 <= code <= 249
   if constexpr (FMT == PF_E4M3) {
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * f, b * f, 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * f, d * f, w, true);

@@ -43,14 +43,14 @@
 // it, which spills, 40%.)
 //
 // Measured (16 heads of 128, e4m3 rows, blocks of 128 tokens, a window of 128):
-//   one token for each of 128 contexts of 512K to 1M tokens  28.8 us + 4.4 the join, for
-//     99.6 MB 3.4 TB/s (a large copy 5.1): bound by the rows' bytes, and by ranges that
-//     end at different times
-//   one token behind 5003, 51 KB  9.6 us: latencies one after another (the step's
-//     arrays, page entries, rows, the waves' join)
-//   up to 2048 tokens behind 64K to 128K in each of 8 sequences  127 to 131 us, 550 TFLOP/s: the
-//     issue of vector instructions beside the products (71 a 16 products, most of them
-//     the softmax; products busy for 38% of the cycles)
+//   one token for each of 128 contexts of 512K to 1M tokens  31 us a call (traced, 28.6 to
+//     31.0 and 4.4 to 4.6 the join), for 99.6 MB 3.2 TB/s (a large copy 5.1): bound by the
+//     rows' bytes, by ranges that end at different times and by the join's launch
+//   one token behind 5003, 51 KB  9.4 us: latencies one after another (the step's
+//     arrays, page entries, rows, the second of a wave's steps, the waves' join)
+//   up to 2048 tokens behind 64K to 128K in each of 8 sequences  116 us a call, 609 TFLOP/s
+//     (130 to 137 under the tracer): the issue of vector instructions beside the products
+//     (77 a 16 products, most of them the softmax; products busy for 35% of the cycles)
 
 #include "paged.h"
 

@@ -776,7 +776,8 @@ class HCAHybridLayer(_FusedWeightLayer):
         of the sequences ``slots`` of ``cache``, packed rows ``x`` ``[N, d]``; what ``forward``
         gives at these positions of the whole sequences. ``residual`` is added.
         ``weight_group`` 32, 64 or 128: the projections run on 4-bit copies of the weights
-        with groups of so many columns (bf16 or fp16 ``x``), made once. Forward only: inputs
+        with groups of so many columns (bf16 or fp16 ``x``), made once (for the few rows of a
+        decode step: a prompt's hundreds of rows run faster without). Forward only: inputs
         that ask for gradients are refused, the layer's own weights are constants."""
         cfg = self.cfg
         c, nh, dc = cfg.hca_c, cfg.hca_nh, cfg.hca_dc

@@ -23,7 +23,8 @@ _GROUPS = (32, 64, 128)
 def linear_w4(x, packed, scales, zeros=None, *, residual=None):
     """``x W^T`` ``[..., N]`` in ``x.dtype`` (bf16 or fp16), plus ``residual``; fp32 sums,
     rounded once. The group is ``K / scales.shape[0]``. Made for the few rows of a decode
-    step; any number is taken, each 16 reading the weights again."""
+    step; any number is taken, each 16 reading the weights again (from 64 rows of a large
+    weight, or 512 of a small one, the 16-bit product is faster)."""
     fn = "linear_w4"
     if not (x.is_cuda and packed.is_cuda):
         _lib.require_gpu(fn, x, packed)
