@@ -10,14 +10,15 @@
 // unnormalised queries and rows scaled by any power of two need and holds the rows of
 // every storage format exactly; fp16, finer by three bits, where the queries are fp16, for
 // what such a model's rows are fits it (paged.h). Scores, sums and outputs are fp32.
-// A query enters as it is, times a power of two: what is left of 1 / ||q|| multiplies the
-// scores with the scale, so a 16-bit query is not rounded again (that alone took a bf16
-// output from 0.0020 off to 0.0026; its own rounding leaves 0.0017). The
-// weights e^(s - M) are rounded to the products' type, as such queries' outputs are. An
-// fp32 query and its weights enter as the three bf16 parts that they are the sums of, three
-// products for one, and its output is off by what fp32 sums are (one bf16 part of each: 2e-3).
-// That takes 48 us a call where bf16 queries take 31 (128 tokens of a batch), 241 where they
-// take 115 (prompt chunks), and as long for short contexts.
+// A query enters as it is, times a power of two, and what is left of 1 / ||q|| multiplies
+// the scores with the scale: a 16-bit query is not rounded again (but for fp16 channels
+// below 2^-14 of the row's length, to 2^-25 of it). A second rounding took a bf16 output
+// from 0.0020 off to 0.0026, where its own rounding leaves 0.0017. The weights
+// e^(s - M) are rounded to the products' type, as such queries' outputs are. An fp32 query
+// and its weights enter as the three bf16 parts that they are the sums of, three products
+// for one, and its output is off by what fp32 sums are (with one bf16 part of each by 2e-3).
+// That takes 48 us a call where bf16 queries take 31 (128 tokens of a batch), 240 where they
+// take 116 (prompt chunks), and no longer for short contexts.
 //
 // All heads share the keys (MQA), so the query rows of a sequence are its tokens
 // times its heads, nh rows a token, and a 16-row MFMA tile may hold rows of

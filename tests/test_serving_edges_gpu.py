@@ -80,6 +80,47 @@ def test_no_token_of_any_chunk(dev, lens):
         assert kch.hca_paged_attention(q, *args, out=mine, **kw) is mine and (mine == 3.0).all()
 
 
+@pytest.mark.parametrize("top", [1, 30])
+def test_captured_padded_step(dev, top):
+    """A captured call that makes its own result, replayed on steps with padding entries: what it held in the replay
+    before does not show, eager work and synchronisations between the replays."""
+    import kch
+    rng = np.random.default_rng(37)
+    S, N, nh, c, m2, win = 4, 3 * top + 5, 16, 64, 16, 16
+    ctx = [9000, 40, 3000, 500]
+    pool = ref.Pool(S, *pages_for([top] * S, ctx, m2, win, 32), 32, c, "int8")
+    fill(pool, [top] * S, ctx, range(S), m2, win, rng)
+    q = torch.zeros(N, nh, c, device="cuda", dtype=torch.bfloat16)
+    s, cu, cx, _ = ref.step([top] * S, ctx, range(S))
+
+    def go():
+        return kch.hca_paged_attention(q, pool.rows, pool.scales, pool.blocks, pool.ring, s, cu, cx, m2=m2,
+                                       sliding_window=win, max_len=top, max_ctx=9000, scale=8.0)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        go()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = go()
+    for lead, lens, slots in ((0, [top, 1, top, 1], [0, 1, 2, 3]), (2, [top, 1, 1, top], [-1, 1, -1, 3]),
+                              (0, [1, 0, 1, 1], [0, -1, 2, 7]), (1, [top] * 3 + [0], [-1] * 4), (0, [1] * 4, [3, 2, 1, 0])):
+        q.copy_(torch.from_numpy(rng.standard_normal(q.shape)))
+        at = lead + np.concatenate([[0], np.cumsum(lens)])
+        s.copy_(torch.tensor(slots)), cu.copy_(torch.tensor(at))
+        cx.copy_(torch.tensor([ctx[k] if 0 <= k < S else 3 for k in slots]))
+        graph.replay()
+        eager = go()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+        answered = torch.zeros(N, dtype=torch.bool, device="cuda")
+        for i, k in enumerate(slots):
+            answered[at[i]:at[i + 1]] = 0 <= k < S
+        assert (out[~answered] == 0).all() and (out[answered].float().abs().amax(-1) > 0).all()
+
+
 # --------------------------------------------------------------------------- masks and rows that are not finite
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
